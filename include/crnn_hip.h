@@ -53,6 +53,7 @@ typedef enum {
 
 #define CRNN_FP32 0
 #define CRNN_BF16 1
+#define CRNN_E4M3 2   /* 8-bit floats (4 exponent bits, 3 mantissa bits, no infinities): operands of crnn_linear, outputs of crnn_rms_norm */
 
 /* Constructor arguments of CRNN(imgH, nc, nclass, nh, leakyRelu, lstmFlag, GPU, alphabet)
  * -- crnn/network_torch.py:37; built at settings.py:45 as CRNN(32,1,nclass,256,False,LSTMFLAG,GPU,alphabet). */
@@ -231,6 +232,105 @@ CRNN_API int crnn_last_timing(crnn_handle* h, float ms[5]);
 CRNN_API int crnn_set_profiling(crnn_handle* h, int32_t on);
 CRNN_API int crnn_last_kernel_times(crnn_handle* h, int32_t cap, const char** names, float* ms,
                                     double* flops, double* bytes);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Operators on sequences of states in device memory: what a decoder that reads several timesteps or lines at once needs
+ * beside the CTC answer.  The reference has no counterpart (its lines are decoded timestep by timestep).
+ *
+ * All pointers in the argument structs are device pointers on the handle's device, except the structs themselves, which
+ * are read during the call.  Strides are in elements.  The work is queued on `stream` (a hipStream_t of that device;
+ * crnn_stream(h, lane) puts it behind that lane's work, NULL is the device's NULL stream) and the call returns without
+ * waiting: nothing is allocated, no stream or event is created and nothing is kept from one call for the next, so calls
+ * may be captured into a HIP graph and made from several threads at once.  The handle gives the device and the error
+ * text (crnn_last_error); it needs no weights.  The first device call of a handle in a process sets its device state up,
+ * which allocates: while `stream` is being captured that is refused with CRNN_ERR_STATE (call crnn_stream(h, 0) before).
+ * An output buffer must not overlap an input except where an argument says so.  Inference only: no gradients.
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* activations of crnn_linear */
+#define CRNN_ACT_NONE 0
+#define CRNN_ACT_RELU 1
+#define CRNN_ACT_LEAKY 2   /* negative slope 0.2, as the network's leakyRelu */
+#define CRNN_ACT_GELU 3    /* x (1 + erf(x / sqrt 2)) / 2 */
+#define CRNN_ACT_SILU 4    /* x / (1 + exp(-x)) */
+
+/* y[i,j] = act( x_scale[i] w_scale[j] sum_k x[i,k] w[j,k] + bias[j] ) + residual[i,j],   i < m, j < n
+ * Sums are fp32.  fp32 operands are multiplied with fp32 accuracy. */
+typedef struct {
+  int64_t m, n, k;           /* m >= 0 (0: nothing to do), n >= 1, k >= 1; each at most 2^31 - 1 */
+  const void* x;             /* [m,k] rows ldx apart, any ldx >= 0 (0: every row the same) */
+  const void* w;             /* [n,k] rows ldw apart (torch's Linear.weight) */
+  int64_t ldx, ldw;
+  const float* x_scale;      /* [m] or NULL (1); CRNN_E4M3 operands only */
+  const float* w_scale;      /* [n] or NULL (1); CRNN_E4M3 operands only */
+  const float* bias;         /* [n] or NULL */
+  const void* residual;      /* [m,n] rows ldr apart, of out_type, or NULL.  May be y itself (same pointer, ldr == ldy) */
+  int64_t ldr;
+  void* y;                   /* [m,n] rows ldy >= n apart */
+  int64_t ldy;
+  int32_t in_type;           /* CRNN_FP32, CRNN_BF16 or CRNN_E4M3: of x and w */
+  int32_t out_type;          /* CRNN_FP32 or CRNN_BF16: of y and residual */
+  int32_t act;               /* CRNN_ACT_* */
+  int32_t reserved;          /* 0 */
+} crnn_linear_args;
+CRNN_API int crnn_linear(crnn_handle* h, const crnn_linear_args* a, void* stream);
+
+/* t = x + residual;  y = t (mean(t^2) + eps)^-1/2 gain, row by row, in fp32; each output is rounded once.
+ * With out_type CRNN_E4M3 every row has a scale c = max(max|y|, 448 * 2^-126) / 448 and y holds the e4m3 values of y / c
+ * (the operands crnn_linear takes).  A NaN or an infinity in a row reaches that row's outputs only. */
+typedef struct {
+  int64_t m, n;              /* rows, row length: m >= 0, n >= 1; each at most 2^31 - 1 */
+  const void* x;             /* [m,n] rows ldx apart, of in_type */
+  int64_t ldx;
+  const void* residual;      /* [m,n] rows ldr apart, of in_type, or NULL */
+  int64_t ldr;
+  const float* gain;         /* [n] */
+  void* sum;                 /* [m,n] rows lds apart, of in_type: t, rounded; or NULL.  May be x or residual themselves */
+  int64_t lds;
+  void* y;                   /* [m,n] rows ldy apart, of out_type.  With out_type == in_type it may be x or residual themselves */
+  int64_t ldy;
+  float* y_scale;            /* [m], with CRNN_E4M3 only; else NULL */
+  float eps;                 /* >= 0 */
+  int32_t in_type;           /* CRNN_FP32 or CRNN_BF16 */
+  int32_t out_type;          /* in_type or CRNN_E4M3 */
+  int32_t reserved;          /* 0 */
+} crnn_rms_norm_args;
+CRNN_API int crnn_rms_norm(crnn_handle* h, const crnn_rms_norm_args* a, void* stream);
+
+/* Attention of queries over an encoder's states of another length:
+ *   s[j] = scale * sum_d q[b,t,h,d] k[b,j,g,d],  p = exp(s - max s),  out[b,t,h,:] = sum_j p[j] v[b,j,g,:] / sum_j p[j]
+ * over the keys j < lengths[b] with mask[b,j] != 0, g = h / (heads / kv_heads).  A row without any key is 0.  Keys that are
+ * left out are never looked at: whatever their k and v hold (infinities, NaN) changes nothing.  Scores, maxima and sums
+ * are fp32; bf16 operands have p rounded to bf16 for the second product. */
+typedef struct {
+  int64_t batch, q_len, kv_len;   /* batch, q_len, kv_len >= 0; kv_len at most 2^31 - 1 */
+  int32_t heads, kv_heads;        /* heads a multiple of kv_heads */
+  int32_t head_dim;               /* 1 .. 128 */
+  int32_t type;                   /* CRNN_FP32 or CRNN_BF16: of q, k, v and out */
+  const void* q;                  /* element (b,t,h,d) at q_stride[0] b + q_stride[1] t + q_stride[2] h + d; likewise: */
+  const void* k;                  /* (b,j,g,d) */
+  const void* v;
+  void* out;                      /* (b,t,h,d) */
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  const int32_t* lengths;         /* [batch] or NULL; values below 0 count as 0, above kv_len as kv_len */
+  const uint8_t* mask;            /* [batch,kv_len] rows mask_stride apart, or NULL */
+  int64_t mask_stride;
+  void* workspace;                /* crnn_cross_attention_workspace bytes, 256-byte aligned, not in use by another call until this one's */
+  int64_t workspace_bytes;        /* work has finished; NULL / 0 where that function answers 0 */
+  float scale;
+  int32_t reserved;               /* 0 */
+} crnn_cross_attention_args;
+CRNN_API int crnn_cross_attention(crnn_handle* h, const crnn_cross_attention_args* a, void* stream);
+/* Bytes of workspace that call needs (0 for most), or a negative status.  Looks at the sizes, the type and the strides only. */
+CRNN_API int64_t crnn_cross_attention_workspace(crnn_handle* h, const crnn_cross_attention_args* a);
+
+/* The recogniser as an encoder: the last recurrent states of n lines (what the classifier reads), for the operators above.
+ * d_gray, n, w, widths as in crnn_forward_device.  d_states [n,T,512], T = crnn_out_len(w), 16-byte aligned: fp32, or bf16 on a CRNN_BF16
+ * handle, zeros from a line's own length on; d_len [n] int32: the lines' lengths, or NULL.  Needs the LSTM head.
+ * Unlike crnn_forward_device the call orders itself against `stream`: the lane that does the work waits for what was queued
+ * on `stream` before, and `stream` waits for the states.  Not under capture (CRNN_ERR_STATE).  Returns the lane. */
+CRNN_API int crnn_states_device(crnn_handle* h, const uint8_t* d_gray, int32_t n, int32_t w, const int32_t* widths,
+                                void* d_states, int32_t* d_len, void* stream);
 
 /* Message of the last failing call on this handle (never NULL). */
 CRNN_API const char* crnn_last_error(const crnn_handle* h);

@@ -14,13 +14,14 @@ LIB_PATH = os.path.join(_PKG, "libcrnn_hip.so")
 CRNN_OK = 0
 CRNN_ERR_ARG, CRNN_ERR_HIP, CRNN_ERR_STATE, CRNN_ERR_ZERO_H, CRNN_ERR_ZERO_W, CRNN_ERR_NOMEM = -1, -2, -3, -4, -5, -6
 PAD_PER_LINE, PAD_REFERENCE = 0, 1
-FP32, BF16 = 0, 1
+FP32, BF16, E4M3 = 0, 1, 2
 
 SYMBOLS = ["crnn_create", "crnn_load_weights", "crnn_resized_width", "crnn_out_len", "crnn_preprocess",
            "crnn_predict_batch", "crnn_set_page", "crnn_predict_rects", "crnn_predict_page", "crnn_forward_device", "crnn_debug_stage", "crnn_synchronize", "crnn_stream", "crnn_lanes",
            "crnn_last_timing", "crnn_set_profiling", "crnn_last_kernel_times", "crnn_last_error", "crnn_destroy",
            "crnn_next_lane", "crnn_split_timeouts", "crnn_forward_device_noalloc", "crnn_noalloc_workspace_bytes",
-           "crnn_channel_scales"]
+           "crnn_channel_scales", "crnn_linear", "crnn_rms_norm", "crnn_cross_attention", "crnn_cross_attention_workspace",
+           "crnn_states_device"]
 
 
 class Config(C.Structure):
@@ -31,6 +32,31 @@ class Config(C.Structure):
 
 class Tensor(C.Structure):
     _fields_ = [("name", C.c_char_p), ("data", C.POINTER(C.c_float)), ("ndim", C.c_int32), ("shape", C.c_int64 * 4)]
+
+
+I64x3 = C.c_int64 * 3
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("x", C.c_void_p), ("w", C.c_void_p), ("ldx", C.c_int64),
+                ("ldw", C.c_int64), ("x_scale", C.c_void_p), ("w_scale", C.c_void_p), ("bias", C.c_void_p),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64), ("in_type", C.c_int32),
+                ("out_type", C.c_int32), ("act", C.c_int32), ("reserved", C.c_int32)]
+
+
+class RmsNormArgs(C.Structure):
+    _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64), ("residual", C.c_void_p),
+                ("ldr", C.c_int64), ("gain", C.c_void_p), ("sum", C.c_void_p), ("lds", C.c_int64), ("y", C.c_void_p),
+                ("ldy", C.c_int64), ("y_scale", C.c_void_p), ("eps", C.c_float), ("in_type", C.c_int32),
+                ("out_type", C.c_int32), ("reserved", C.c_int32)]
+
+
+class CrossAttentionArgs(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("q_len", C.c_int64), ("kv_len", C.c_int64), ("heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("type", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("out", C.c_void_p), ("q_stride", I64x3), ("k_stride", I64x3), ("v_stride", I64x3),
+                ("out_stride", I64x3), ("lengths", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("scale", C.c_float), ("reserved", C.c_int32)]
 
 
 _lib = None
@@ -173,6 +199,16 @@ def lib():
     L.crnn_noalloc_workspace_bytes.argtypes = [vp, i32, i32]
     L.crnn_channel_scales.restype = C.c_int
     L.crnn_channel_scales.argtypes = [vp, i32, C.POINTER(C.c_float), i32]
+    L.crnn_linear.restype = C.c_int
+    L.crnn_linear.argtypes = [vp, C.POINTER(LinearArgs), vp]
+    L.crnn_rms_norm.restype = C.c_int
+    L.crnn_rms_norm.argtypes = [vp, C.POINTER(RmsNormArgs), vp]
+    L.crnn_cross_attention.restype = C.c_int
+    L.crnn_cross_attention.argtypes = [vp, C.POINTER(CrossAttentionArgs), vp]
+    L.crnn_cross_attention_workspace.restype = C.c_int64
+    L.crnn_cross_attention_workspace.argtypes = [vp, C.POINTER(CrossAttentionArgs)]
+    L.crnn_states_device.restype = C.c_int
+    L.crnn_states_device.argtypes = [vp, vp, i32, i32, vp, vp, vp, vp]
     _lib = L
     return L
 

@@ -14,6 +14,7 @@ import os
 import numpy as np
 
 from . import _capi
+from .seq_ops import SequenceOps
 from .util import labels_to_text
 
 
@@ -34,7 +35,7 @@ def _as_gray_array(image):
     return a
 
 
-class CRNN(object):
+class CRNN(SequenceOps):
     """Same surface as ``crnn.network_torch.CRNN``; inference only."""
 
     def __init__(self, imgH, nc, nclass, nh, leakyRelu=False, lstmFlag=True, GPU=False, alphabet=None, device=None,

@@ -4,6 +4,7 @@
 // entry point fails with CRNN_ERR_HIP.
 #include "../../include/crnn_hip.h"
 #include "crnn_kernels.h"
+#include "crnn_seq.h"
 
 #include <unistd.h>
 
@@ -62,6 +63,7 @@ constexpr int MAXK = 48;
 struct Lane {
   hipStream_t stream = nullptr;
   hipEvent_t ev[5] = {nullptr, nullptr, nullptr, nullptr, nullptr};
+  hipEvent_t order = nullptr;  // crnn_states_device: orders the lane and the caller's stream
   bool ev_valid = false;
   hipEvent_t kev[MAXK + 1] = {};
   const char* kname[MAXK] = {};
@@ -285,6 +287,7 @@ int ensure_device(crnn_handle* h, bool need_weights = true) {
       Lane& L = h->lanes[l];
       HIPCHK(h, hipStreamCreateWithFlags(&L.stream, hipStreamNonBlocking));
       for (int i = 0; i < 5; i++) HIPCHK(h, hipEventCreate(&L.ev[i]));
+      HIPCHK(h, hipEventCreateWithFlags(&L.order, hipEventDisableTiming));
       for (int i = 0; i <= MAXK; i++) HIPCHK(h, hipEventCreate(&L.kev[i]));
     }
     upload_norm_lut(h->lut, tl_cur->stream);
@@ -298,6 +301,7 @@ int ensure_device(crnn_handle* h, bool need_weights = true) {
       launch_warm_main(ls);
       launch_warm_bf16(ls);
       launch_warm_nopk(ls);
+      launch_warm_seq(ls);
       HIPCHK(h, hipMemsetAsync(h->d_zero_bias, 0, 16, ls));
       HIPCHK(h, hipEventRecord(h->lanes[l].ev[0], ls));
       HIPCHK(h, hipStreamSynchronize(ls));
@@ -345,6 +349,44 @@ int ensure_device(crnn_handle* h, bool need_weights = true) {
   }
   return 0;
 }
+
+}  // namespace
+
+namespace crnn {
+
+SeqDevice::~SeqDevice() {
+  if (before >= 0) (void)hipSetDevice(before);
+}
+
+int seq_fail(crnn_handle* h, int code, const char* msg) { return fail(h, code, msg); }
+
+int seq_enter(crnn_handle* h, void* stream, SeqDevice* dev, bool need_weights, bool locked) {
+  std::unique_lock<std::mutex> lk(h->mu, std::defer_lock);
+  if (!locked) lk.lock();
+  int cur = -1;
+  HIPCHK(h, hipGetDevice(&cur));
+  const bool ready = h->dev_ready && h->dev_pid == getpid() && (!need_weights || h->weights_on_dev);
+  if (ready && !need_weights) {   // (the common case: nothing but the device to set)
+    if (cur != h->cfg.device) {
+      HIPCHK(h, hipSetDevice(h->cfg.device));
+      dev->before = cur;
+    }
+    return 0;
+  }
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  if (stream) HIPCHK(h, hipStreamIsCapturing((hipStream_t)stream, &cs));
+  if (cs != hipStreamCaptureStatusNone)
+    return fail(h, CRNN_ERR_STATE, need_weights ? "not while the stream is being captured"
+                                                : "the device state of this handle does not exist yet and may not be made while the "
+                                                  "stream is being captured: call crnn_stream(h, 0) before");
+  dev->before = cur;
+  tl_cur = &h->lanes[0];
+  return ensure_device(h, need_weights);
+}
+
+}  // namespace crnn
+
+namespace {
 
 // ---- Pillow Resample.c coefficient computation (BILINEAR, support 1.0) ------
 // Same double-precision expressions as precompute_coeffs / normalize_coeffs_8bpc
@@ -684,7 +726,8 @@ int conv(crnn_handle* h, int layer, const void* A, void* C, const int32_t* wvali
 // per-line valid widths or nullptr.  Outputs (device): plan.raw plus d_lab/d_len.
 // allow_split: the caller synchronises afterwards and checks split_timed_out() (host paths only)
 int run_network(crnn_handle* h, const Geo& g, const Plan& p, const int32_t* widths, int32_t* d_lab,
-                int32_t* d_len, bool want_logits = false, bool allow_split = false, bool may_alloc = true) {
+                int32_t* d_len, bool want_logits = false, bool allow_split = false, bool may_alloc = true,
+                void* d_states = nullptr) {
   const int n = g.n;
   const int act = h->cfg.leaky_relu ? 2 : 1;
   const int32_t *m_p0 = nullptr, *m_c1 = nullptr, *m_w2 = nullptr, *m_w3 = nullptr, *tlen = nullptr;
@@ -841,6 +884,16 @@ int run_network(crnn_handle* h, const Geo& g, const Plan& p, const int32_t* widt
     gemm(h, "lstm1_ih", p.mid, h->d_wih[1], h->db_wih[1], h->d_bih[1], p.xp, M, 2048, 256, false, nullptr, nullptr,
          h->d_wih_h3[1], h->wih_us[1], p.a3, p.rs);
     rec(1, p.rec1);
+    if (d_states) {   // crnn_states_device: no classifier (d_len: the lines' lengths, may be null)
+      launch_copy_states(p.rec1, d_states, d_len, tlen, n, g.T, b16, s);
+      kmark(h, "copy_states", 0, 2.0 * es * M * 512);
+      HIPCHK(h, hipEventRecord(tl_cur->ev[3], s));
+      HIPCHK(h, hipEventRecord(tl_cur->ev[4], s));
+      tl_cur->ev_valid = true;
+      h->last.store(tl_cur, std::memory_order_release);
+      HIPCHK(h, hipGetLastError());
+      return 0;
+    }
     filtered = classify(p.rec1, h->d_emb_w[1], h->db_emb_w[1], h->d_emb_b[1]);
   } else {
     filtered = classify(p.seq, h->d_lin_w, h->db_lin_w, h->d_lin_b);
@@ -1616,6 +1669,53 @@ int crnn_forward_device(crnn_handle* h, const uint8_t* d_gray, int32_t n, int32_
   return lane;
 }
 
+int crnn_states_device(crnn_handle* h, const uint8_t* d_gray, int32_t n, int32_t w, const int32_t* widths,
+                       void* d_states, int32_t* d_len, void* stream) {
+  if (!h) return CRNN_ERR_ARG;
+  try {
+    std::lock_guard<std::mutex> lk(h->mu);
+    if (!d_gray || n <= 0 || w < 8 || !d_states) return fail(h, CRNN_ERR_ARG, "bad arguments");
+    if (((uintptr_t)d_states & 15) || ((uintptr_t)d_len & 3)) return fail(h, CRNN_ERR_ARG, "d_states is not 16-byte aligned, or d_len not to its type");
+    if (!h->cfg.lstm) return fail(h, CRNN_ERR_STATE, "crnn_states_device: a handle without the LSTM head has no recurrent states");
+    if (widths)
+      for (int i = 0; i < n; i++)
+        if (widths[i] < 8 || widths[i] > w) return fail(h, CRNN_ERR_ARG, "line width outside [8, w]");
+    SeqDevice dev;
+    int rc = seq_enter(h, stream, &dev, true, true);
+    if (rc) return rc;
+    const int lane = h->next_lane;
+    h->next_lane = (h->next_lane + 1) % h->nlanes;
+    Lane& L = h->lanes[lane];
+    tl_cur = &L;
+    std::lock_guard<std::mutex> lane_lk(L.mu);
+    const Geo g(n, w);
+    Plan p;
+    if ((rc = prepare_plan(h, g, p))) return rc;
+    HIPCHK(h, hipEventRecord(L.order, (hipStream_t)stream));
+    HIPCHK(h, hipStreamWaitEvent(L.stream, L.order, 0));
+    int32_t* d_w = nullptr;
+    if (widths) {
+      d_w = p.wl + 4 * (size_t)n;
+      HIPCHK(h, hipMemcpyAsync(d_w, widths, sizeof(int32_t) * n, hipMemcpyHostToDevice, L.stream));
+    }
+    HIPCHK(h, hipEventRecord(L.ev[0], L.stream));
+    L.nk = 0;
+    if (h->kprof) HIPCHK(h, hipEventRecord(L.kev[0], L.stream));
+    launch_normalize(d_gray, p.x, d_w, n, w, w, L.stream);
+    kmark(h, "normalize", 0, (double)n * 32 * w * 5.0);
+    L.pblocks = 256;
+    if ((rc = run_network(h, g, p, widths, nullptr, d_len, false, false, true, d_states))) {
+      (void)hipStreamSynchronize(L.stream);   // the caller may free the buffers: nothing of a half-queued run is left behind
+      return rc;
+    }
+    HIPCHK(h, hipEventRecord(L.order, L.stream));
+    HIPCHK(h, hipStreamWaitEvent((hipStream_t)stream, L.order, 0));
+    return lane;
+  } catch (const std::exception& e) {
+    return fail(h, CRNN_ERR_NOMEM, e.what());
+  }
+}
+
 int64_t crnn_noalloc_workspace_bytes(const crnn_handle* h, int32_t n, int32_t w) {
   if (!h || n <= 0 || w < 8) return CRNN_ERR_ARG;
   return (int64_t)make_plan(h, Geo(n, w), nullptr).bytes;
@@ -1828,6 +1928,7 @@ void crnn_destroy(crnn_handle* h) {
       (void)hipFree(L.arena.p); (void)hipFree(L.pre.p); (void)hipFree(L.io.p); (void)hipHostFree(L.stage.p);
       (void)hipFree(L.page.p); (void)hipFree(L.sync.p);
       for (int i = 0; i < 5; i++) (void)hipEventDestroy(L.ev[i]);
+      (void)hipEventDestroy(L.order);
       for (int i = 0; i <= MAXK; i++) (void)hipEventDestroy(L.kev[i]);
       (void)hipStreamDestroy(L.stream);
     }

@@ -1,0 +1,162 @@
+"""Argument checks of the sequence operators and the error bounds their tests use: no GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from ocr_amd.crnn import _capi
+from tests import seq_reference as R
+
+
+@pytest.fixture(scope="module")
+def handle():
+    lib = _capi.lib()
+    h = C.c_void_p()
+    cfg = _capi.Config(32, 1, 65, 256, 0, 1, 0, 1, 0, 0)
+    assert lib.crnn_create(C.byref(cfg), C.byref(h)) == 0
+    yield lib, h
+    lib.crnn_destroy(h)
+
+
+def fields(struct, a, **change):
+    d = dict(a, **change)
+    return struct(*[d[n] for n, _ in struct._fields_])
+
+
+P = 1 << 32      # a pointer that is never followed: every call here is refused, or has nothing to do
+LIN = dict(m=4, n=8, k=16, x=P, w=P + 4096, ldx=16, ldw=16, x_scale=None, w_scale=None, bias=P + 8192, residual=None, ldr=0, y=P + 16384, ldy=8,
+           in_type=_capi.BF16, out_type=_capi.BF16, act=0, reserved=0)
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(x=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"), (dict(m=-1), "range"), (dict(n=0), "range"), (dict(k=0), "range"),
+    (dict(m=1 << 31), "range"), (dict(in_type=3), "in_type"), (dict(out_type=_capi.E4M3), "out_type"), (dict(act=5), "activation"),
+    (dict(act=-1), "activation"), (dict(ldy=7), "ldy"), (dict(ldx=-1), "stride"), (dict(ldw=-1), "stride"), (dict(x_scale=P + 9000), "scales"),
+    (dict(x=P + 1), "aligned"), (dict(bias=P + 8193), "aligned"), (dict(y=P), "overlaps"), (dict(y=P + 4096), "overlaps"), (dict(y=P + 8192), "overlaps"),
+    (dict(residual=P + 16386, ldr=8), "residual"), (dict(residual=P + 16384, ldr=9), "residual"), (dict(reserved=1), "reserved"),
+    (dict(y=P + 16, ldx=24, ldy=24, n=9), "overlaps"),      # columns 8..16 of the buffer whose columns 0..15 are x
+])
+def test_linear_refuses(handle, change, word):
+    lib, h = handle
+    a = fields(_capi.LinearArgs, LIN, **change)
+    assert lib.crnn_linear(h, C.byref(a), None) == _capi.CRNN_ERR_ARG
+    assert word in lib.crnn_last_error(h).decode()
+
+
+NORM = dict(m=4, n=16, x=P, ldx=16, residual=P + 4096, ldr=16, gain=P + 8192, sum=P + 12288, lds=16, y=P + 16384, ldy=16, y_scale=None, eps=1e-6,
+            in_type=_capi.BF16, out_type=_capi.BF16, reserved=0)
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(x=None), "null"), (dict(gain=None), "null"), (dict(y=None), "null"), (dict(m=-1), "range"), (dict(n=0), "range"), (dict(eps=-1.0), "eps"),
+    (dict(eps=float("nan")), "eps"), (dict(in_type=_capi.E4M3), "in_type"), (dict(out_type=_capi.FP32), "out_type"), (dict(y_scale=P + 20000), "y_scale"),
+    (dict(out_type=_capi.E4M3), "y_scale"), (dict(ldy=15), "overlap"), (dict(lds=15), "overlap"), (dict(ldx=-2), "stride"), (dict(x=P + 1), "aligned"),
+    (dict(y=P + 2), "overlaps an input"), (dict(y=P, ldy=17), "overlaps an input"), (dict(sum=P + 16384), "two outputs"), (dict(y=P + 8192), "overlaps an input"),
+    (dict(reserved=7), "reserved"), (dict(out_type=_capi.E4M3, y_scale=P + 20000, y=P), "overlaps an input"),
+])
+def test_rms_norm_refuses(handle, change, word):
+    lib, h = handle
+    a = fields(_capi.RmsNormArgs, NORM, **change)
+    assert lib.crnn_rms_norm(h, C.byref(a), None) == _capi.CRNN_ERR_ARG
+    assert word in lib.crnn_last_error(h).decode()
+
+
+ATT = dict(batch=2, q_len=3, kv_len=5, heads=4, kv_heads=2, head_dim=8, type=_capi.BF16, q=P, k=P + 4096, v=P + 8192, out=P + 16384,
+           q_stride=_capi.I64x3(96, 32, 8), k_stride=_capi.I64x3(80, 16, 8), v_stride=_capi.I64x3(80, 16, 8), out_stride=_capi.I64x3(96, 32, 8),
+           lengths=None, mask=None, mask_stride=0, workspace=None, workspace_bytes=0, scale=0.3, reserved=0)
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(q=None), "null"), (dict(k=None), "null"), (dict(v=None), "null"), (dict(out=None), "null"), (dict(heads=3), "multiple"), (dict(heads=0), "multiple"),
+    (dict(kv_heads=0), "multiple"), (dict(head_dim=0), "head_dim"), (dict(head_dim=129), "head_dim"), (dict(batch=-1), "range"), (dict(kv_len=1 << 31), "range"),
+    (dict(batch=1 << 20, q_len=1 << 20), "passes"), (dict(type=_capi.E4M3), "type"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(q_stride=_capi.I64x3(-1, 0, 0)), "stride"), (dict(out_stride=_capi.I64x3(96, 32, 7)), "rows of out"), (dict(out_stride=_capi.I64x3(95, 32, 8)), "rows of out"),
+    (dict(out_stride=_capi.I64x3(0, 32, 8)), "rows of out"), (dict(out=P), "overlaps q"), (dict(out=P + 4096), "overlaps k"), (dict(out=P + 8192), "overlaps k"),
+    (dict(mask=P + 16400, mask_stride=5), "mask"), (dict(mask=P, mask_stride=-1), "mask_stride"), (dict(lengths=P + 16388), "lengths"), (dict(lengths=P + 2), "aligned"),
+    (dict(q=P + 1), "aligned"), (dict(reserved=1), "reserved"),
+])
+def test_cross_attention_refuses(handle, change, word):
+    lib, h = handle
+    a = fields(_capi.CrossAttentionArgs, ATT, **change)
+    assert lib.crnn_cross_attention(h, C.byref(a), None) == _capi.CRNN_ERR_ARG
+    assert word in lib.crnn_last_error(h).decode()
+
+
+def test_nothing_to_do_is_no_error(handle):
+    lib, h = handle
+    assert lib.crnn_linear(h, C.byref(fields(_capi.LinearArgs, LIN, m=0, x=None, y=None)), None) == 0
+    assert lib.crnn_rms_norm(h, C.byref(fields(_capi.RmsNormArgs, NORM, m=0, x=None)), None) == 0
+    for none in (dict(batch=0), dict(q_len=0)):
+        a = fields(_capi.CrossAttentionArgs, ATT, q=None, **none)
+        assert lib.crnn_cross_attention(h, C.byref(a), None) == 0 and lib.crnn_cross_attention_workspace(h, C.byref(a)) == 0
+
+
+def test_null_arguments(handle):
+    lib, h = handle
+    for f in (lib.crnn_linear, lib.crnn_rms_norm, lib.crnn_cross_attention):
+        assert f(h, None, None) == _capi.CRNN_ERR_ARG and f(None, None, None) == _capi.CRNN_ERR_ARG
+    assert lib.crnn_cross_attention_workspace(h, None) == _capi.CRNN_ERR_ARG
+    assert lib.crnn_states_device(h, None, 1, 64, None, None, None, None) == _capi.CRNN_ERR_ARG
+    assert lib.crnn_states_device(h, P, 1, 64, None, P + 8, None, None) == _capi.CRNN_ERR_ARG
+
+
+def test_tensors_of_the_host_are_refused():
+    from ocr_amd.crnn.network_hip import CRNN
+    m = CRNN(32, 1, 65, 256, device=0)
+    x = torch.zeros(2, 16)
+    for call in (lambda: m.linear(x, x), lambda: m.rms_norm(x, x[0]), lambda: m.cross_attention(x.view(1, 2, 2, 8), x.view(1, 2, 2, 8), x.view(1, 2, 2, 8)),
+                 lambda: m.line_states(torch.zeros(1, 32, 64, dtype=torch.uint8))):
+        with pytest.raises(ValueError, match="on cpu"):
+            call()
+    with pytest.raises(TypeError):
+        m.linear(x.numpy(), x)
+
+
+def test_line_attention_checks_its_weights():
+    from ocr_amd.crnn.attention import LineAttention
+    w = {"norm.weight": torch.ones(64), "q.weight": torch.zeros(32, 64), "kv.weight": torch.zeros(64, 512), "out.weight": torch.zeros(64, 32)}
+    assert LineAttention(None, w, heads=4).d == 8
+    for bad in (dict(w, extra=w["norm.weight"]), {k: v for k, v in w.items() if k != "out.weight"}, dict(w, **{"kv.weight": torch.zeros(64, 511)}),
+                dict(w, **{"q.weight": w["q.weight"].bfloat16()}), dict(w, **{"q.scale": torch.ones(32)}), dict(w, **{"norm.weight": torch.ones(63)})):
+        with pytest.raises(ValueError):
+            LineAttention(None, bad, heads=4)
+    with pytest.raises(ValueError):
+        LineAttention(None, w, heads=4, kv_heads=3)
+
+
+def test_rows_of_a_tensor():
+    from ocr_amd.crnn.seq_ops import SequenceOps
+    rows = SequenceOps._rows
+    t = torch.zeros(6, 5, 32)
+    assert rows("f", "t", t, 32) == (30, 32) and rows("f", "t", t[:, 0], 32) == (6, 160) and rows("f", "t", t[:, :, :16], 16) == (30, 32)
+    assert rows("f", "t", t[0, 0], 32) == (1, 32) and rows("f", "t", t[:, :0], 32)[0] == 0 and rows("f", "t", t[:1, 2:3], 32) == (1, 32)
+    assert rows("f", "t", t[0, :1].expand(7, 32), 32) == (7, 0)
+    with pytest.raises(ValueError):
+        rows("f", "t", t[:, :4], 32)
+    with pytest.raises(ValueError):
+        rows("f", "t", t, 16)
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "leaky", "gelu", "silu"])
+def test_the_linear_bound_holds_for_32_bit_sums_and_not_for_a_mistake(act):
+    g = torch.Generator().manual_seed(1)
+    x, w, b = torch.randn(9, 70, generator=g), torch.randn(13, 70, generator=g), torch.randn(13, generator=g)
+    want, err = R.linear(x, w, b, act=act)
+    got = R.act64((x @ w.t() + b), act)
+    R.check(got, want, err)
+    w2 = w.clone()
+    w2[3, 69] = 0
+    with pytest.raises(AssertionError):
+        R.check(R.act64(x @ w2.t() + b, act), want, err)
+
+
+def test_the_attention_bound_holds_for_32_bits_and_not_for_a_lost_key():
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(2, n, 4, 8, generator=g) for n in (3, 50, 50))
+    want, err = R.attention(q, k, v, lengths=torch.tensor([50, 17]))
+    z = torch.einsum("bthd,bshd->bhts", q, k) * 8 ** -0.5
+    z[1, :, :, 17:] = -float("inf")
+    R.check(torch.einsum("bhts,bshd->bthd", torch.softmax(z, 3), v), want, err)
+    z[1, :, :, 16:] = -float("inf")
+    with pytest.raises(AssertionError):
+        R.check(torch.einsum("bhts,bshd->bthd", torch.softmax(z, 3), v), want, err)
