@@ -1,6 +1,7 @@
 // Kernels of the sequence operators (include/crnn_hip.h: crnn_linear, crnn_rms_norm, crnn_cross_attention), gfx950.
 // Compiled without packed fp32 (crnn_kernels_nopk.hip says why).
 #include "crnn_seq.h"
+#include "crnn_kernels.h"
 
 #include <cmath>
 
@@ -10,6 +11,10 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned char e4m3;   // the byte of an e4m3 value
 
 // Workgroups of a launch: a grid of 2^24 workgroups of 256 would pass the 2^32 threads a launch may have, so the kernels
@@ -452,10 +457,345 @@ __global__ __launch_bounds__(256, 2) void attention_any_kernel(const crnn_cross_
   }
 }
 
-int64_t cross_attention_workspace(const crnn_cross_attention_args&) { return 0; }
+// Direct loads from memory into LDS: lane l's 16 bytes at `voff` land at `lds` + 16 l; offsets past the resource give zeros.
+// The compiler does not count them: every use of the data is behind a wait of its own.
+__device__ __forceinline__ void dma16(i32x4 rsrc, unsigned lds, unsigned voff) {
+  unsigned m0_saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0_saved) : "s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+constexpr unsigned OUTSIDE = 0x80000000u;   // past every resource below
+__device__ __forceinline__ i32x4 resource(const void* p) {
+  const unsigned long long u = (unsigned long long)p;
+  return i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)u), (int)(__builtin_amdgcn_readfirstlane((unsigned)(u >> 32)) & 0xFFFF), 0x7FFFFFFF, 0x00020000};
+}
+
+// bf16, head_dim and strides in whole 16-byte chunks.  Four waves (or one): RW of them side by side over 32 rows each, KW of
+// them over different tiles of KT keys; head_dim padded to DP.  Both products run transposed, S^T = K Q^T and O^T = V^T P^T
+// (v_mfma_f32_32x32x16_bf16): a lane then holds one query row in both results, so maximum, sum and rescaling are per lane, and
+// the exponentials are the second product's operand as they stand, because its sum may run over the keys in any order: register
+// r of S^T is key (r & 3) + 8 (r >> 2) + 4 (lane >> 5), and ds_read_tr16_b64 takes V's columns for four such keys at a time.
+// K and V tiles go straight to LDS, two stages; 16-byte chunk c of row j sits at chunk c ^ swizzle(j), which spreads the eight
+// rows (K) or the four half rows (V) that are read at once over all banks.  Keys that are left out are never loaded: their
+// offset lies outside the resource, LDS gets zeros, and their score is -inf.
+// With nsplit > 1 workgroups share the keys of one row block and leave (O, M, L) for attention_join_kernel.
+struct AttnPlan {
+  int rw, kw, nsplit;
+};
+
+template <int DP, int RW, int KW, int KT>
+__global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const crnn_cross_attention_args a, int nsplit) {
+  constexpr int NCH = DP / 8, ROWB = DP * 2, TILE = KT * ROWB, NW = RW * KW;   // chunks of a row, bytes of a row and of a tile
+  constexpr int LOADS = TILE / 1024;                                          // dma16 instructions a tile, shared by RW waves
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[KW * 4 * TILE];   // [KW][2 stages][K, V]
+  static_assert(KW == 1 || sizeof(smem) >= (RW * DP * 32 + RW * 64) * 4, "the join's exchange fits the tiles");
+  if constexpr (sizeof(smem) > 80 * 1024) CRNN_WHOLE_REGISTER_FILE();   // (one workgroup a CU: the compiler uses AccVGPRs)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int kw = wave / RW, rw = wave % RW;
+  const int G = a.heads / a.kv_heads, D = a.head_dim;
+  const int64_t rows = a.q_len * G, nrb = (rows + 32 * RW - 1) / (32 * RW), total = a.batch * a.kv_heads * nrb * nsplit;
+  // consecutive blocks (row blocks and splits of one key head) on one XCD, whose L2 then holds their keys
+  const int64_t per = (total + 7) / 8, blk = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (blk >= total || (blockIdx.x >> 3) >= per) return;
+  const int sp = (int)(blk % nsplit);
+  const int64_t rb = blk / nsplit % nrb, bg = blk / nsplit / nrb, b = bg / a.kv_heads, g = bg % a.kv_heads;
+  const int len = a.lengths ? max(0, (int)min((int64_t)a.lengths[b], a.kv_len)) : (int)a.kv_len;
+  // this workgroup's keys: whole steps of KW tiles
+  const int steps_all = (len + KT * KW - 1) / (KT * KW), steps_per = (steps_all + nsplit - 1) / nsplit;
+  const int step0 = min(sp * steps_per, steps_all), steps = min(steps_per, steps_all - step0);
+  const __bf16* kp = (const __bf16*)a.k + b * a.k_stride[0] + g * a.k_stride[2];
+  const __bf16* vp = (const __bf16*)a.v + b * a.v_stride[0] + g * a.v_stride[2];
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
+
+  // query rows, as the second operand: lane & 31 the row, 8 values from 16 kk + 8 half.  A negative scale turns their sign
+  const float sc = fmaxf(fabsf(a.scale), 1e-38f) * 1.4426950408889634f;
+  const int64_t row = rb * 32 * RW + rw * 32 + (lane & 31);
+  const bool live = row < rows;
+  bf16x8 q[DP / 16];
+  {
+    const __bf16* qp = (const __bf16*)a.q + b * a.q_stride[0] + (live ? row / G : 0) * a.q_stride[1] + (g * G + (live ? row % G : 0)) * a.q_stride[2];
+    const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; kk++) {
+      const int d = 16 * kk + 8 * half;
+      i32x4 u = {0, 0, 0, 0};
+      if (live && d < D) u = *(const i32x4*)(qp + d);
+#pragma unroll
+      for (int i = 0; i < 4; i++) u[i] ^= flip;
+      q[kk] = __builtin_bit_cast(bf16x8, u);
+    }
+  }
+  auto swz_k = [](int r) { return NCH % 8 == 0 ? r & 7 : (r >> 1) & 3; };
+  auto swz_v = [](int r) { return NCH % 8 == 0 ? 2 * (r & 3) : 2 * ((r >> 1) & 1); };
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem + kw * 4 * TILE;
+  const unsigned char* base = smem + kw * 4 * TILE;
+
+  // keys that count in tile `t` of this key wave, one bit each
+  auto bits_of = [&](int step, int mbyte) __attribute__((always_inline)) -> unsigned long long {
+    const int j0 = (step * KW + kw) * KT;
+    unsigned long long w = len - j0 >= 64 ? ~0ull : len - j0 <= 0 ? 0ull : (1ull << (len - j0)) - 1;
+    if (KT < 64) w &= (1ull << (KT & 63)) - 1;
+    if (mask) w &= __ballot(mbyte != 0);
+    return w;
+  };
+  auto mask_byte = [&](int step) __attribute__((always_inline)) -> int {
+    const int j = (step * KW + kw) * KT + lane;
+    return mask && (KT == 64 || lane < KT) && j < len ? mask[j] : 0;
+  };
+  auto load = [&](int step, int stage, unsigned long long w) __attribute__((always_inline)) {
+    if (w == 0) return;
+    const int64_t j0 = (int64_t)(step * KW + kw) * KT;
+    const i32x4 rk = resource(kp + j0 * a.k_stride[1]), rv = resource(vp + j0 * a.v_stride[1]);
+#pragma unroll
+    for (int i = 0; i < (LOADS + RW - 1) / RW; i++) {
+      const int n = i * RW + rw;
+      if (LOADS % RW != 0 && n >= LOADS) break;
+      const int pos = n * 64 + lane, r = pos / NCH, c = pos % NCH;
+      const bool key = (w >> r) & 1;
+      const int ck = c ^ swz_k(r), cv = c ^ swz_v(r);
+      dma16(rk, lds0 + stage * 2 * TILE + n * 1024, key && ck * 8 < D ? (unsigned)(r * (int)a.k_stride[1] + ck * 8) * 2u : OUTSIDE);
+      dma16(rv, lds0 + stage * 2 * TILE + TILE + n * 1024, key && cv * 8 < D ? (unsigned)(r * (int)a.v_stride[1] + cv * 8) * 2u : OUTSIDE);
+    }
+  };
+
+  f32x16 o[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) o[i][r] = 0.f;
+  float M = -INFINITY, L = 0.f;   // M in units of the raw score; L of this half-wave's keys only, joined at the end
+
+  unsigned long long w0 = 0, w1 = 0;
+  if (steps > 0) {
+    w0 = bits_of(step0, mask_byte(step0));
+    load(step0, 0, w0);
+    if (steps > 1) w1 = bits_of(step0 + 1, mask_byte(step0 + 1));
+  }
+  for (int it = 0; it < steps; it++) {
+    const int st = it & 1;
+    int mb = 0;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // this step's tiles are in LDS, the last one's reads done
+    if (RW > 1) __syncthreads();                       // ... of all waves, and the other stage is no longer read
+    if (it + 1 < steps) load(step0 + it + 1, st ^ 1, w1);
+    if (it + 2 < steps) mb = mask_byte(step0 + it + 2);
+    const unsigned long long w = w0;
+    if (w != 0) {
+      const unsigned char* kt = base + st * 2 * TILE;
+      const unsigned char* vt = kt + TILE;
+      f32x16 s[KT / 32];
+#pragma unroll
+      for (int kb = 0; kb < KT / 32; kb++) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[kb][r] = 0.f;
+        const int r = kb * 32 + (lane & 31);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; kk++) {
+          const bf16x8 f = *(const bf16x8*)(kt + r * ROWB + (((2 * kk + half) ^ swz_k(r)) << 4));
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, q[kk], s[kb], 0, 0, 0);
+        }
+      }
+      const unsigned long long full = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
+      if (w != full) {
+        const unsigned long long wl = w >> (4 * half);
+#pragma unroll
+        for (int kb = 0; kb < KT / 32; kb++)
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            if (!((wl >> (kb * 32 + (r & 3) + 8 * (r >> 2))) & 1)) s[kb][r] = -INFINITY;
+      }
+      float mt = s[0][0];
+#pragma unroll
+      for (int kb = 0; kb < KT / 32; kb++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[kb][r]);
+      mt = fmaxf(mt, __shfl_xor(mt, 32));
+      const float Mn = fmaxf(M, mt), Ms = Mn == -INFINITY ? 0.f : Mn * sc;
+      if (__any(Mn > M)) {   // (wave-uniform: most tiles after the first few raise no row's maximum)
+        const float al = __builtin_amdgcn_exp2f(M * sc - Ms);
+        L *= al;
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[i][r] *= al;
+        M = Mn;
+      }
+#pragma unroll
+      for (int kb = 0; kb < KT / 32; kb++) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], sc, -Ms));
+          L += s[kb][r];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          bf16x8 pj;
+#pragma unroll
+          for (int i = 0; i < 8; i++) pj[i] = (__bf16)s[kb][8 * j + i];
+#pragma unroll
+          for (int db = 0; db < DP / 32; db++) {
+            s16x4 f[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int r = kb * 32 + 16 * j + 8 * i + 4 * half + ((lane & 15) >> 2), c = db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+              f[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + r * ROWB + ((c ^ swz_v(r)) << 4) + (lane & 1) * 8));
+            }
+            const s16x8 v8 = __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v8), pj, o[db], 0, 0, 0);
+          }
+        }
+      }
+    }
+    w0 = w1;
+    if (it + 2 < steps) w1 = bits_of(step0 + it + 2, mb);
+  }
+  L += __shfl_xor(L, 32);
+  // M in exponent units from here on
+  float Me = M * sc;
+  if constexpr (KW > 1) {   // join the key waves of a row block: through LDS, one wave after the other
+    float* xo = (float*)smem;                       // [RW][DP][32]
+    float* xm = xo + RW * DP * 32;                  // [RW][2][32]
+    for (int w = 1; w < KW; w++) {
+      __syncthreads();
+      if (kw == w) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) xo[(rw * DP + i * 32 + acc_row(r, lane)) * 32 + (lane & 31)] = o[i][r];
+        if (half == 0) xm[(rw * 2) * 32 + lane] = Me, xm[(rw * 2 + 1) * 32 + lane] = L;
+      }
+      __syncthreads();
+      if (kw == 0) {
+        const float m2 = xm[(rw * 2) * 32 + (lane & 31)], l2 = xm[(rw * 2 + 1) * 32 + (lane & 31)];
+        const float mn = fmaxf(Me, m2), ms = mn == -INFINITY ? 0.f : mn;
+        const float a1 = __builtin_amdgcn_exp2f(Me - ms), a2 = __builtin_amdgcn_exp2f(m2 - ms);
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[i][r] = o[i][r] * a1 + xo[(rw * DP + i * 32 + acc_row(r, lane)) * 32 + (lane & 31)] * a2;
+        L = L * a1 + l2 * a2;
+        Me = mn;
+      }
+    }
+    if (kw != 0) return;
+  }
+  if (!live) return;
+  if (nsplit > 1) {
+    // [split][row of all blocks][D values, M, L] fp32
+    float* ws = (float*)a.workspace + ((int64_t)sp * (a.batch * a.kv_heads * rows) + bg * rows + row) * (D + 2);
+#pragma unroll
+    for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int d = i * 32 + acc_row(r, lane);
+        if (d < D) ws[d] = o[i][r];
+      }
+    if (half == 0) ws[D] = Me, ws[D + 1] = L;
+    return;
+  }
+  __bf16* out = (__bf16*)a.out + b * a.out_stride[0] + row / G * a.out_stride[1] + (g * G + row % G) * a.out_stride[2];
+  const float il = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = i * 32 + acc_row(r, lane);   // four neighbours; head_dim is a multiple of 8
+      if (d < D) *(bf16x4u*)(out + d) = bf16x4u{(__bf16)(o[i][r] * il), (__bf16)(o[i][r + 1] * il), (__bf16)(o[i][r + 2] * il), (__bf16)(o[i][r + 3] * il)};
+    }
+}
+
+// out = sum_s O_s 2^(M_s - M) / sum_s L_s 2^(M_s - M), a thread per value of out
+template <int TYPE>
+__global__ __launch_bounds__(256) void attention_join_kernel(const crnn_cross_attention_args a, int nsplit) {
+  typedef typename TypeOf<TYPE>::t T;
+  const int G = a.heads / a.kv_heads, D = a.head_dim;
+  const int64_t rows = a.q_len * G, all = a.batch * a.kv_heads * rows, total = all * D;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / D, bg = r / rows, row = r - bg * rows;
+    const int d = (int)(i - r * D);
+    const float* ws = (const float*)a.workspace + r * (D + 2);
+    float M = -INFINITY, L = 0.f, o = 0.f;
+    for (int s = 0; s < nsplit; s++) M = fmaxf(M, ws[s * all * (D + 2) + D]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    for (int s = 0; s < nsplit; s++) {
+      const float* w = ws + s * all * (D + 2);
+      const float e = exp2f(w[D] - Ms);
+      L += w[D + 1] * e;
+      o += w[d] * e;
+    }
+    T* out = (T*)a.out + bg / a.kv_heads * a.out_stride[0] + row / G * a.out_stride[1] + (bg % a.kv_heads * G + row % G) * a.out_stride[2];
+    out[d] = (T)(L == 0.f ? 0.f : o / L);
+  }
+}
+
+static bool attention_chunks(const crnn_cross_attention_args& a) {   // (sizes, type and strides only)
+  if (a.type != CRNN_BF16 || a.head_dim % 8 != 0 || a.kv_len == 0) return false;
+  for (int i = 0; i < 3; i++)
+    if (a.q_stride[i] % 8 != 0 || a.k_stride[i] % 8 != 0 || a.v_stride[i] % 8 != 0) return false;
+  return a.k_stride[1] < (1 << 23) && a.v_stride[1] < (1 << 23);   // a tile's offsets stay below 2^31 bytes
+}
+static bool attention_aligned(const crnn_cross_attention_args& a) { return (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0; }
+
+static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
+  const int64_t rows = a.q_len * (a.heads / a.kv_heads), bg = a.batch * a.kv_heads;
+  AttnPlan p;
+  p.rw = rows > 64 ? 4 : rows > 32 ? 2 : 1;
+  p.kw = 4 / p.rw;
+  const int kt = p.rw == 4 ? 64 : 32;
+  if (p.rw == 1 && a.kv_len <= 4 * kt && bg >= 1024) p.kw = 1;   // few keys, many heads: a wave a head, nothing to join
+  const int64_t blocks = bg * ((rows + 32 * p.rw - 1) / (32 * p.rw)), steps = (a.kv_len + kt * p.kw - 1) / (kt * p.kw);
+  int64_t ns = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
+  ns = ns < steps / 2 ? ns : steps / 2;                            // at least two steps each
+  p.nsplit = (int)(ns < 1 ? 1 : ns > 256 ? 256 : ns);
+  return p;
+}
+
+int64_t cross_attention_workspace(const crnn_cross_attention_args& a) {
+  if (!attention_chunks(a)) return 0;
+  const AttnPlan p = attention_plan(a);
+  return p.nsplit <= 1 ? 0 : (int64_t)p.nsplit * a.batch * a.heads * a.q_len * (a.head_dim + 2) * 4;
+}
+
+template <int DP, int RW, int KW>
+static void attention_bf16(const crnn_cross_attention_args& a, int nsplit, hipStream_t s) {
+  constexpr int KT = RW == 4 ? 64 : 32;
+  const int64_t rows = a.q_len * (a.heads / a.kv_heads), total = a.batch * a.kv_heads * ((rows + 32 * RW - 1) / (32 * RW)) * nsplit;
+  hipLaunchKernelGGL((attention_bf16_kernel<DP, RW, KW, KT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * RW * KW), 0, s, a, nsplit);
+}
+template <int DP>
+static void attention_bf16(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
+  if (p.rw == 4) attention_bf16<DP, 4, 1>(a, p.nsplit, s);
+  else if (p.rw == 2) attention_bf16<DP, 2, 2>(a, p.nsplit, s);
+  else if (p.kw == 4) attention_bf16<DP, 1, 4>(a, p.nsplit, s);
+  else attention_bf16<DP, 1, 1>(a, p.nsplit, s);
+}
 
 void launch_cross_attention(const crnn_cross_attention_args& a, hipStream_t s) {
   const int64_t rows = a.q_len * (a.heads / a.kv_heads);
+  const int64_t blocks = a.batch * a.kv_heads * ((rows + 31) / 32);
+  if (attention_chunks(a) && attention_aligned(a) && (blocks < (1 << 22) || a.batch > 1)) {
+    if (blocks >= 1 << 22) {   // a launch has fewer than 2^32 threads: half the batch at a time (so many blocks use no workspace)
+      crnn_cross_attention_args h[2] = {a, a};
+      const int64_t n = a.batch / 2;
+      h[0].batch = n;
+      h[1].batch = a.batch - n;
+      h[1].q = (const __bf16*)a.q + n * a.q_stride[0];
+      h[1].k = (const __bf16*)a.k + n * a.k_stride[0];
+      h[1].v = (const __bf16*)a.v + n * a.v_stride[0];
+      h[1].out = (__bf16*)a.out + n * a.out_stride[0];
+      if (a.lengths) h[1].lengths = a.lengths + n;
+      if (a.mask) h[1].mask = a.mask + n * a.mask_stride;
+      launch_cross_attention(h[0], s);
+      launch_cross_attention(h[1], s);
+      return;
+    }
+    const AttnPlan p = attention_plan(a);
+    if (a.head_dim <= 32) attention_bf16<32>(a, p, s);
+    else if (a.head_dim <= 64) attention_bf16<64>(a, p, s);
+    else if (a.head_dim <= 96) attention_bf16<96>(a, p, s);
+    else attention_bf16<128>(a, p, s);
+    if (p.nsplit > 1) hipLaunchKernelGGL((attention_join_kernel<CRNN_BF16>), grid_for((a.batch * a.heads * a.q_len * a.head_dim + 255) / 256), dim3(256), 0, s, a, p.nsplit);
+    return;
+  }
   const dim3 g = grid_for(a.batch * a.kv_heads * ((rows + 15) / 16)), b(256);
   if (a.type == CRNN_FP32) hipLaunchKernelGGL((attention_any_kernel<CRNN_FP32>), g, b, 0, s, a);
   else hipLaunchKernelGGL((attention_any_kernel<CRNN_BF16>), g, b, 0, s, a);
