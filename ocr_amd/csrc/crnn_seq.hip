@@ -15,6 +15,7 @@ typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned char e4m3;   // the byte of an e4m3 value
 
 // Workgroups of a launch: a grid of 2^24 workgroups of 256 would pass the 2^32 threads a launch may have, so the kernels
@@ -37,6 +38,65 @@ __device__ __forceinline__ float activate(float v, int act) {
     case CRNN_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
     case CRNN_ACT_SILU: return v / (1.f + expf(-v));
     default: return v;
+  }
+}
+
+// Eight neighbouring values of a row of whole 16-byte chunks.
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+}
+__device__ __forceinline__ void load8(const __bf16* p, float (&v)[8]) {
+  const bf16x8 a = *(const bf16x8*)p;
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  *(f32x4*)p = f32x4{v[0], v[1], v[2], v[3]};
+  *(f32x4*)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+}
+__device__ __forceinline__ void store8(__bf16* p, const float (&v)[8]) {
+  bf16x8 a;
+#pragma unroll
+  for (int i = 0; i < 8; i++) a[i] = (__bf16)v[i];
+  *(bf16x8*)p = a;
+}
+__device__ __forceinline__ void store8(e4m3* p, const float (&v)[8]) {
+  i32x2 a;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
+    a[i] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], u, true);
+  }
+  *(i32x2*)p = a;
+}
+
+// Direct loads from memory into LDS: lane l's 16 bytes at `voff` + `soff` land at `lds` + 16 l; offsets past the resource give zeros.
+// The compiler does not count them: every use of the data is behind a wait of its own.
+__device__ __forceinline__ void dma16(i32x4 rsrc, unsigned lds, unsigned voff, unsigned soff = 0) {
+  unsigned m0_saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0_saved) : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
+}
+constexpr unsigned OUTSIDE = 0x80000000u;   // past every resource below
+__device__ __forceinline__ i32x4 resource(const void* p) {
+  const unsigned long long u = (unsigned long long)p;
+  return i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)u), (int)(__builtin_amdgcn_readfirstlane((unsigned)(u >> 32)) & 0xFFFF), 0x7FFFFFFF, 0x00020000};
+}
+
+__device__ __forceinline__ void activate8(float (&v)[8], int act) {
+  if (act == CRNN_ACT_NONE) return;
+  if (act == CRNN_ACT_GELU) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = activate(v[e], CRNN_ACT_GELU);
+  } else if (act == CRNN_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = activate(v[e], CRNN_ACT_SILU);
+  } else {
+    const float slope = act == CRNN_ACT_LEAKY ? 0.2f : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = v[e] > 0.f ? v[e] : act == CRNN_ACT_RELU ? 0.f : slope * v[e];
   }
 }
 
@@ -105,18 +165,247 @@ __global__ __launch_bounds__(256, 2) void linear_any_kernel(const crnn_linear_ar
   }
 }
 
-void launch_linear(const crnn_linear_args& a, hipStream_t s) {
-  const dim3 g = grid_for((a.m + 63) / 64 * ((a.n + 63) / 64)), b(256);
-  if (a.in_type == CRNN_FP32) {
-    if (a.out_type == CRNN_FP32) hipLaunchKernelGGL((linear_any_kernel<CRNN_FP32, CRNN_FP32>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((linear_any_kernel<CRNN_FP32, CRNN_BF16>), g, b, 0, s, a);
-  } else if (a.in_type == CRNN_BF16) {
-    if (a.out_type == CRNN_FP32) hipLaunchKernelGGL((linear_any_kernel<CRNN_BF16, CRNN_FP32>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((linear_any_kernel<CRNN_BF16, CRNN_BF16>), g, b, 0, s, a);
-  } else {
-    if (a.out_type == CRNN_FP32) hipLaunchKernelGGL((linear_any_kernel<CRNN_E4M3, CRNN_FP32>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((linear_any_kernel<CRNN_E4M3, CRNN_BF16>), g, b, 0, s, a);
+// ---------------------------------------------------------------------------
+// linear, rows of whole 16-byte chunks (bf16, and e4m3 with bf16 results): a tile of 64 NT columns x 64 MT rows of y per
+// workgroup of four waves (2 x 2), a step of 128 bytes of k of every row at a time, straight from memory into two LDS stages.
+// 16-byte chunk c of row r sits at chunk c ^ (r & 7): the eight rows read at once by ds_read_b128 cover all banks.  w is the first
+// operand, so that a lane holds four neighbouring columns of one row of y (v_mfma_f32_32x32x16_bf16; 8 bits:
+// v_mfma_f32_32x32x64_f8f6f4, 32 bytes a lane).
+// A step has NKS slices of matrix instructions; each slice's operands are read during the slice before.  One barrier a step,
+// before its last slice: by then the other stage has landed and nobody reads this one any more, so the loads for the step
+// after next go out during the last slice and the first one of the next step.
+// ---------------------------------------------------------------------------
+template <int IN> struct Slice;
+template <> struct Slice<CRNN_BF16> {
+  static constexpr int NKS = 4, CH = 1;   // slices of a step; 16-byte chunks of a lane's operand
+  typedef i32x4 frag;
+  static __device__ __forceinline__ frag read(const unsigned char* row, int ks, int half, int swz) { return *(const i32x4*)(row + (((2 * ks + half) ^ swz) << 4)); }
+  static __device__ __forceinline__ f32x16 mfma(frag w, frag x, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x), c, 0, 0, 0);
   }
+};
+template <> struct Slice<CRNN_E4M3> {
+  static constexpr int NKS = 2, CH = 2;
+  typedef i32x8 frag;
+  static __device__ __forceinline__ frag read(const unsigned char* row, int ks, int half, int swz) {
+    const int c = 4 * ks + 2 * half;
+    const i32x4 a = *(const i32x4*)(row + ((c ^ swz) << 4)), b = *(const i32x4*)(row + (((c + 1) ^ swz) << 4));
+    return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+  static __device__ __forceinline__ f32x16 mfma(frag w, frag x, f32x16 c) { return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, 0, 0, 0, 0); }
+};
+
+// Eight values of a row of y: residual, rounding, store.  `n8` of them exist; `wide`: rows of 16-byte chunks.
+template <typename TO>
+__device__ __forceinline__ void put8(const crnn_linear_args& a, int64_t m, int64_t n, int n8, bool wide, float (&v)[8]) {
+  TO* y = (TO*)a.y + m * a.ldy + n;
+  const TO* r = a.residual ? (const TO*)a.residual + m * a.ldr + n : nullptr;
+  if (wide && n8 >= 8) {
+    if (r) {
+      float t[8];
+      load8(r, t);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] += t[i];
+    }
+    store8(y, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i < n8) y[i] = (TO)(r ? v[i] + (float)r[i] : v[i]);
+  }
+}
+
+template <int IN, int OUT, int MT, int NT>
+__global__ __launch_bounds__(256, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a, int wide) {
+  typedef Slice<IN> S;
+  typedef typename TypeOf<OUT>::t TO;
+  constexpr int ES = IN == CRNN_BF16 ? 2 : 1, NKS = S::NKS;
+  constexpr int BM = 64 * MT, BN = 64 * NT, STAGE = (BM + BN) * 128;
+  constexpr int LX = BM / 32, LW = BN / 32, LT = LX + LW;   // dma16 instructions of a wave and step
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
+  static_assert(sizeof(smem) >= 4 * 32 * (32 * NT * 4 + 16), "the epilogue's exchange fits");
+  if constexpr (MT * NT > 8) CRNN_WHOLE_REGISTER_FILE();
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int wm = wave >> 1, wn = wave & 1;
+  // Tiles in groups of eight rows of tiles, column by column; a run of consecutive tiles per XCD, so that the 32 tiles it works
+  // on at a time are 8 x 4 and share their operands in its L2
+  const int ntm = (int)((a.m + BM - 1) / BM), ntn = (int)((a.n + BN - 1) / BN), total = ntm * ntn;
+  const int per = (total + 7) / 8, t0 = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (t0 >= total) return;
+  const int grp = t0 / (8 * ntn), in = t0 - grp * 8 * ntn, gm = min(8, ntm - grp * 8);
+  const int64_t m0 = (int64_t)(grp * 8 + in % gm) * BM, n0 = (int64_t)(in / gm) * BN;
+
+  const unsigned kbytes = (unsigned)a.k * ES;
+  const int nk = (int)((kbytes + 127) / 128);
+  const i32x4 rx = resource((const char*)a.x + m0 * a.ldx * ES), rw = resource((const char*)a.w + n0 * a.ldw * ES);
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
+  // lane l of load i of this wave: row (wave + 4 i) 8 + l / 8, chunk (l & 7) ^ (row & 7) = (l & 7) ^ (l >> 3)
+  const unsigned cb = (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
+  unsigned ox[LX], ow[LW];
+#pragma unroll
+  for (int i = 0; i < LX; i++) {
+    const int r = (wave + 4 * i) * 8 + (lane >> 3);
+    ox[i] = m0 + r < a.m ? (unsigned)(r * (int)a.ldx * ES) + cb : OUTSIDE;
+  }
+#pragma unroll
+  for (int i = 0; i < LW; i++) {
+    const int r = (wave + 4 * i) * 8 + (lane >> 3);
+    ow[i] = n0 + r < a.n ? (unsigned)(r * (int)a.ldw * ES) + cb : OUTSIDE;
+  }
+  auto load = [&](int step, int i) __attribute__((always_inline)) {   // load i of LT: x before w
+    const unsigned s = lds0 + (step & 1) * STAGE, kb = (unsigned)step * 128;
+    const unsigned off = i < LX ? ox[i] : ow[i - LX], to = i < LX ? (wave + 4 * i) * 1024 : BM * 128 + (wave + 4 * (i - LX)) * 1024;
+    dma16(i < LX ? rx : rw, s + to, kb + cb < kbytes ? off : OUTSIDE, kb);   // (past the end of a row: zeros)
+  };
+  f32x16 acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; i++)
+#pragma unroll
+    for (int j = 0; j < MT; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+  typename S::frag fx[2][MT], fw[2][NT];
+  const int swz = lane & 7;
+  const unsigned char* xrow = smem + (wm * 32 * MT + (lane & 31)) * 128;
+  const unsigned char* wrow = smem + BM * 128 + (wn * 32 * NT + (lane & 31)) * 128;
+  auto read_x = [&](int set, int stage, int ks, int j) __attribute__((always_inline)) { fx[set][j] = S::read(xrow + stage * STAGE + j * 4096, ks, half, swz); };
+  auto read_w = [&](int set, int stage, int ks, int i) __attribute__((always_inline)) { fw[set][i] = S::read(wrow + stage * STAGE + i * 4096, ks, half, swz); };
+
+#pragma unroll
+  for (int i = 0; i < LT; i++) load(0, i);
+  if (nk > 1) {
+#pragma unroll
+    for (int i = 0; i < LT; i++) load(1, i);
+    if (LT == 16) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    else if (LT == 12) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  static_assert(LT == 16 || LT == 12 || LT == 8, "the wait above");
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < MT; j++) read_x(0, 0, 0, j);
+#pragma unroll
+  for (int i = 0; i < NT; i++) read_w(0, 0, 0, i);
+#pragma unroll 1
+  for (int t = 0; t < nk; t++) {
+    const int st = t & 1;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ks++) {
+      const int set = ks & 1, last = ks == NKS - 1;
+      if (last) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NT; i++) {
+        // operands of the next slice (after the last step: of a stage that is not read any more)
+        read_w(set ^ 1, last ? st ^ 1 : st, last ? 0 : ks + 1, i);
+        if (NT == MT) read_x(set ^ 1, last ? st ^ 1 : st, last ? 0 : ks + 1, i);
+        else if (NT < MT) {
+          read_x(set ^ 1, last ? st ^ 1 : st, last ? 0 : ks + 1, 2 * i);
+          read_x(set ^ 1, last ? st ^ 1 : st, last ? 0 : ks + 1, 2 * i + 1);
+        } else if (i % 2 == 0) {
+          read_x(set ^ 1, last ? st ^ 1 : st, last ? 0 : ks + 1, i / 2);
+        }
+        constexpr int PER = LT / 2 / NT;
+        if (last && t + 2 < nk) {
+#pragma unroll
+          for (int l = 0; l < PER; l++) load(t + 2, i * PER + l);
+        }
+        if (ks == 0 && t > 0 && t + 1 < nk) {
+#pragma unroll
+          for (int l = 0; l < PER; l++) load(t + 1, LT / 2 + i * PER + l);
+        }
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[i][j] = S::mfma(fw[set][i], fx[set][j], acc[i][j]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  // Epilogue: the sums of 32 rows at a time go through LDS (each wave has its own part), after which a lane holds eight
+  // neighbours of a row: bias, activation and residual happen there, and rows leave as whole lines.
+  __syncthreads();   // (nobody reads the stages any more)
+  constexpr int PITCH = 32 * NT * 4 + 16;
+  constexpr int LPR = 4 * NT, RPI = 64 / LPR;   // lanes a row, rows at a time
+  unsigned char* ex = smem + wave * 32 * PITCH;
+  const int c = (lane % LPR) * 8;
+  const int64_t n = n0 + wn * 32 * NT + c, left = a.n - n;
+  float bias[8], wsc[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    bias[e] = a.bias && e < left ? a.bias[n + e] : 0.f;
+    wsc[e] = IN == CRNN_E4M3 && a.w_scale && e < left ? a.w_scale[n + e] : 1.f;
+  }
+#pragma unroll
+  for (int j = 0; j < MT; j++) {
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+      for (int g = 0; g < 4; g++)
+        *(f32x4*)(ex + (lane & 31) * PITCH + (i * 32 + 8 * g + 4 * half) * 4) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int r = lane / LPR; r < 32; r += RPI) {
+      const f32x4 lo = *(const f32x4*)(ex + r * PITCH + c * 4), hi = *(const f32x4*)(ex + r * PITCH + c * 4 + 16);
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      const int64_t m = m0 + wm * 32 * MT + j * 32 + r;
+      if (m < a.m && left > 0) {
+        const float sx = IN == CRNN_E4M3 && a.x_scale ? a.x_scale[m] : 1.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = IN == CRNN_E4M3 ? v[e] * sx * wsc[e] + bias[e] : v[e] + bias[e];
+        activate8(v, a.act);
+        put8<TO>(a, m, n, left < 8 ? (int)left : 8, wide, v);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Rows of whole 16-byte chunks, and offsets within a tile below 2^31 bytes.
+static bool linear_chunks(const crnn_linear_args& a) {
+  const int64_t es = a.in_type == CRNN_BF16 ? 2 : 1, c = 16 / es;
+  if (a.in_type == CRNN_FP32 || (a.in_type == CRNN_E4M3 && a.out_type == CRNN_FP32)) return false;
+  return a.k % c == 0 && a.ldx % c == 0 && a.ldw % c == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 &&
+         (256 * (a.ldx > a.ldw ? a.ldx : a.ldw) + a.k) * es < 0x7FFFFFFF;
+}
+
+template <int IN, int OUT, int MT, int NT>
+static void linear_tile(const crnn_linear_args& a, hipStream_t s) {
+  const int64_t eo = OUT == CRNN_FP32 ? 4 : 2;
+  auto chunks = [&](const void* p, int64_t ld) { return (((uintptr_t)p | (uintptr_t)(ld * eo)) & 15) == 0; };
+  const int wide = chunks(a.y, a.ldy) && (!a.residual || chunks(a.residual, a.ldr));
+  const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 64 * NT - 1) / (64 * NT));
+  hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), 0, s, a, wide);
+}
+template <int IN, int OUT>
+static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
+  if ((a.m + 63) / 64 * ((a.n + 63) / 64) >= 1 << 23) return false;   // (a launch has fewer than 2^32 threads)
+  const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
+  if (big >= 192) linear_tile<IN, OUT, 4, 4>(a, s);
+  else linear_tile<IN, OUT, 2, 2>(a, s);
+  return true;
+}
+
+template <int IN, int OUT>
+static void linear_of(const crnn_linear_args& a, hipStream_t s) {
+  if constexpr (IN == CRNN_BF16 || (IN == CRNN_E4M3 && OUT == CRNN_BF16)) {
+    if (linear_chunks(a) && linear_tiles<IN, OUT>(a, s)) return;
+  }
+  hipLaunchKernelGGL((linear_any_kernel<IN, OUT>), grid_for((a.m + 63) / 64 * ((a.n + 63) / 64)), dim3(256), 0, s, a);
+}
+
+void launch_linear(const crnn_linear_args& a, hipStream_t s) {
+  if (a.in_type == CRNN_FP32) a.out_type == CRNN_FP32 ? linear_of<CRNN_FP32, CRNN_FP32>(a, s) : linear_of<CRNN_FP32, CRNN_BF16>(a, s);
+  else if (a.in_type == CRNN_BF16) a.out_type == CRNN_FP32 ? linear_of<CRNN_BF16, CRNN_FP32>(a, s) : linear_of<CRNN_BF16, CRNN_BF16>(a, s);
+  else a.out_type == CRNN_FP32 ? linear_of<CRNN_E4M3, CRNN_FP32>(a, s) : linear_of<CRNN_E4M3, CRNN_BF16>(a, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -227,36 +516,6 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(const crnn_rms_norm_a
 // Rows of 16-byte chunks that fit the registers of one wave (TPR 64: four rows a workgroup) or one workgroup (TPR 256): x and
 // the residual are read once, everything else happens in registers.  A thread holds C groups of eight values; the gain stays in
 // registers over the rows that a workgroup takes.  Bound by HBM.
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-#pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
-}
-__device__ __forceinline__ void load8(const __bf16* p, float (&v)[8]) {
-  const bf16x8 a = *(const bf16x8*)p;
-#pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = (float)a[i];
-}
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  *(f32x4*)p = f32x4{v[0], v[1], v[2], v[3]};
-  *(f32x4*)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-}
-__device__ __forceinline__ void store8(__bf16* p, const float (&v)[8]) {
-  bf16x8 a;
-#pragma unroll
-  for (int i = 0; i < 8; i++) a[i] = (__bf16)v[i];
-  *(bf16x8*)p = a;
-}
-__device__ __forceinline__ void store8(e4m3* p, const float (&v)[8]) {
-  i32x2 a;
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
-    a[i] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], u, true);
-  }
-  *(i32x2*)p = a;
-}
-
 template <int IN, int OUT, int TPR, int C>
 __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args a) {
   typedef typename TypeOf<IN>::t T;
@@ -455,19 +714,6 @@ __global__ __launch_bounds__(256, 2) void attention_any_kernel(const crnn_cross_
       if (d < D) out[d] = (T)(o[i] * il);
     }
   }
-}
-
-// Direct loads from memory into LDS: lane l's 16 bytes at `voff` land at `lds` + 16 l; offsets past the resource give zeros.
-// The compiler does not count them: every use of the data is behind a wait of its own.
-__device__ __forceinline__ void dma16(i32x4 rsrc, unsigned lds, unsigned voff) {
-  unsigned m0_saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0_saved) : "s"(lds), "v"(voff), "s"(rsrc) : "memory");
-}
-constexpr unsigned OUTSIDE = 0x80000000u;   // past every resource below
-__device__ __forceinline__ i32x4 resource(const void* p) {
-  const unsigned long long u = (unsigned long long)p;
-  return i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)u), (int)(__builtin_amdgcn_readfirstlane((unsigned)(u >> 32)) & 0xFFFF), 0x7FFFFFFF, 0x00020000};
 }
 
 // bf16, head_dim and strides in whole 16-byte chunks.  Four waves (or one): RW of them side by side over 32 rows each, KW of

@@ -28,7 +28,8 @@ def randn(g, *shape, dt="fp32"):
 
 # ------------------------------------------------------------------------------------------------------- linear
 SIZES = [(1, 512, 512), (1, 7, 3), (2, 64, 5530), (3, 33, 65), (7, 517, 129), (16, 2048, 64), (17, 8200, 48), (48, 512, 5530), (64, 128, 33), (130, 96, 260),
-         (71, 1, 1), (255, 512, 511), (300, 1000, 256), (513, 256, 2048), (1000, 64, 70), (257, 4096, 512), (2500, 576, 640), (5000, 513, 255)]
+         (71, 1, 1), (255, 512, 511), (300, 1000, 256), (513, 256, 2048), (1000, 64, 70), (257, 4096, 512), (2500, 576, 640), (5000, 513, 255),
+         (12500, 264, 1025), (17000, 80, 770), (3000, 1040, 4100)]
 
 
 def linear_inputs(m, k, n, dt, seed):
