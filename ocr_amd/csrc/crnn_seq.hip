@@ -51,6 +51,9 @@ __device__ __forceinline__ float activate(float v, int act) {
 }
 
 // Eight neighbouring values of a row of whole 16-byte chunks.
+template <typename T> struct Eight;
+template <> struct Eight<float> { typedef float t __attribute__((ext_vector_type(8), aligned(16))); };
+template <> struct Eight<__bf16> { typedef __bf16 t __attribute__((ext_vector_type(8))); };
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
   const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
 #pragma unroll
@@ -94,18 +97,18 @@ __device__ __forceinline__ i32x4 resource(const void* p) {
   return i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)u), (int)(__builtin_amdgcn_readfirstlane((unsigned)(u >> 32)) & 0xFFFF), 0x7FFFFFFF, 0x00020000};
 }
 
-__device__ __forceinline__ void activate8(float (&v)[8], int act) {
-  if (act == CRNN_ACT_NONE) return;
+template <int N>
+__device__ __forceinline__ void activate_all(float (&v)[N], int act) {
   if (act == CRNN_ACT_GELU) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = gelu(v[e]);
+    for (int e = 0; e < N; e++) v[e] = gelu(v[e]);
   } else if (act == CRNN_ACT_SILU) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = silu(v[e]);
-  } else {
+    for (int e = 0; e < N; e++) v[e] = silu(v[e]);
+  } else if (act != CRNN_ACT_NONE) {
     const float slope = act == CRNN_ACT_LEAKY ? 0.2f : 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = v[e] > 0.f ? v[e] : act == CRNN_ACT_RELU ? 0.f : slope * v[e];
+    for (int e = 0; e < N; e++) v[e] = v[e] > 0.f ? v[e] : act == CRNN_ACT_RELU ? 0.f : slope * v[e];
   }
 }
 
@@ -176,17 +179,17 @@ __global__ __launch_bounds__(256, 2) void linear_any_kernel(const crnn_linear_ar
 
 // ---------------------------------------------------------------------------
 // linear, rows of whole 16-byte chunks (bf16, and e4m3 with bf16 results): a tile of 64 NT columns x 64 MT rows of y per
-// workgroup of four waves (2 x 2), a step of 128 bytes of k of every row at a time, straight from memory into two LDS stages.
-// 16-byte chunk c of row r sits at chunk c ^ (r & 7): the eight rows read at once by ds_read_b128 cover all banks.  w is the first
-// operand, so that a lane holds four neighbouring columns of one row of y (v_mfma_f32_32x32x16_bf16; 8 bits:
-// v_mfma_f32_32x32x64_f8f6f4, 32 bytes a lane).
-// A step has NKS slices of matrix instructions; each slice's operands are read during the slice before.  One barrier a step,
-// before its last slice: by then the other stage has landed and nobody reads this one any more, so the loads for the step
-// after next go out during the last slice and the first one of the next step.
+// workgroup of four waves (2 x 2), a step of 64 bytes of k of every row at a time, straight from memory into one of NST LDS
+// stages.  16-byte chunk c of row r sits at chunk c ^ ((r >> 2) & 3): the 16 rows that ds_read_b128 reads at once are then 16
+// different parts of the 256 bytes that LDS serves in a cycle.  w is the first operand, so that a lane holds four neighbouring
+// columns of one row of y (v_mfma_f32_32x32x16_bf16, two slices a step; 8 bits: v_mfma_f32_32x32x64_f8f6f4, one slice).
+// Each slice's operands are read during the slice before.  One barrier a step, in its last slice: by then everybody has read
+// this step's stage, and the loads for NST steps on go into it; what bounds the loop is their way from memory, so the stages
+// take all of LDS.  Steps past the end load zeros, which keeps the count of loads in flight the same to the last step.
 // ---------------------------------------------------------------------------
 template <int IN> struct Slice;
 template <> struct Slice<CRNN_BF16> {
-  static constexpr int NKS = 4, CH = 1;   // slices of a step; 16-byte chunks of a lane's operand
+  static constexpr int KB = 32;   // bytes of k of a slice
   typedef i32x4 frag;
   static __device__ __forceinline__ frag read(const unsigned char* row, int ks, int half, int swz) { return *(const i32x4*)(row + (((2 * ks + half) ^ swz) << 4)); }
   static __device__ __forceinline__ f32x16 mfma(frag w, frag x, f32x16 c) {
@@ -194,7 +197,7 @@ template <> struct Slice<CRNN_BF16> {
   }
 };
 template <> struct Slice<CRNN_E4M3> {
-  static constexpr int NKS = 2, CH = 2;
+  static constexpr int KB = 64;
   typedef i32x8 frag;
   static __device__ __forceinline__ frag read(const unsigned char* row, int ks, int half, int swz) {
     const int c = 4 * ks + 2 * half;
@@ -204,67 +207,61 @@ template <> struct Slice<CRNN_E4M3> {
   static __device__ __forceinline__ f32x16 mfma(frag w, frag x, f32x16 c) { return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, 0, 0, 0, 0); }
 };
 
-// Eight values of a row of y: residual, rounding, store.  `n8` of them exist; `wide`: rows of 16-byte chunks.
+// Up to eight values of a row of y, one by one: residual, rounding, store.
 template <typename TO>
-__device__ __forceinline__ void put8(const crnn_linear_args& a, int64_t m, int64_t n, int n8, bool wide, float (&v)[8]) {
+__device__ __forceinline__ void put(const crnn_linear_args& a, int64_t m, int64_t n, int count, const float (&v)[8]) {
   TO* y = (TO*)a.y + m * a.ldy + n;
   const TO* r = a.residual ? (const TO*)a.residual + m * a.ldr + n : nullptr;
-  if (wide && n8 >= 8) {
-    if (r) {
-      float t[8];
-      load8(r, t);
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] += t[i];
-    }
-    store8(y, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (i < n8) y[i] = (TO)(r ? v[i] + (float)r[i] : v[i]);
-  }
+  for (int i = 0; i < 8; i++)
+    if (i < count) y[i] = (TO)(r ? v[i] + (float)r[i] : v[i]);
 }
 
-template <int IN, int OUT, int MT, int NT>
-__global__ __launch_bounds__(256, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a, int wide) {
+template <int N> __device__ __forceinline__ void wait_loads() {   // all but the last N loads have landed; LDS reads done
+  static_assert(N < 64, "vmcnt has six bits");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST>
+__global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a, int wide) {
   typedef Slice<IN> S;
   typedef typename TypeOf<OUT>::t TO;
-  constexpr int ES = IN == CRNN_BF16 ? 2 : 1, NKS = S::NKS;
-  constexpr int BM = 64 * MT, BN = 64 * NT, STAGE = (BM + BN) * 128;
-  constexpr int LX = BM / 32, LW = BN / 32, LT = LX + LW;   // dma16 instructions of a wave and step
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
-  static_assert(sizeof(smem) >= 4 * 32 * (32 * NT * 4 + 16), "the epilogue's exchange fits");
+  constexpr int ES = IN == CRNN_BF16 ? 2 : 1, NKS = RB / S::KB, RPL = 1024 / RB;   // slices of a step, rows of a load
+  constexpr int NW = 2 * WN, BM = 64 * MT, BN = 32 * WN * NT, STAGE = (BM + BN) * RB;
+  constexpr int LX = BM / (RPL * NW), LT = (BM + BN) / (RPL * NW);   // dma16 instructions of a wave and step: of x, all
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[NST * STAGE];
+  static_assert(sizeof(smem) >= NW * 32 * (32 * NT * 4 + 16), "the epilogue's exchange fits");
   if constexpr (MT * NT > 8) CRNN_WHOLE_REGISTER_FILE();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / WN, wn = wave % WN;
   // Tiles in groups of eight rows of tiles, column by column; a run of consecutive tiles per XCD, so that the 32 tiles it works
   // on at a time are 8 x 4 and share their operands in its L2
   const int ntm = (int)((a.m + BM - 1) / BM), ntn = (int)((a.n + BN - 1) / BN), total = ntm * ntn;
   const int per = (total + 7) / 8, t0 = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (t0 >= total) return;
+  if (t0 >= total || (int)(blockIdx.x >> 3) >= per) return;
   const int grp = t0 / (8 * ntn), in = t0 - grp * 8 * ntn, gm = min(8, ntm - grp * 8);
   const int64_t m0 = (int64_t)(grp * 8 + in % gm) * BM, n0 = (int64_t)(in / gm) * BN;
 
   const unsigned kbytes = (unsigned)a.k * ES;
-  const int nk = (int)((kbytes + 127) / 128);
+  const int nk = (int)((kbytes + RB - 1) / RB);
   const i32x4 rx = resource((const char*)a.x + m0 * a.ldx * ES), rw = resource((const char*)a.w + n0 * a.ldw * ES);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
-  // lane l of load i of this wave: row (wave + 4 i) 8 + l / 8, chunk (l & 7) ^ (row & 7) = (l & 7) ^ (l >> 3)
-  const unsigned cb = (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
-  unsigned ox[LX], ow[LW];
+  // lane l of load i of this wave: row r = (wave + NW i) RPL + l / (RB / 16), chunk (l mod RB / 16) ^ swizzle(r), the same for all i
+  auto swizzle = [](int r) { return RB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; };
+  const int lr = lane / (RB / 16);
+  const unsigned cb = (unsigned)(((lane & (RB / 16 - 1)) ^ swizzle(wave * RPL + lr)) * 16);
+  static_assert(NW * RPL % 16 == 0, "a load's rows start at the same place of the swizzle");
+  unsigned off[LT];
 #pragma unroll
-  for (int i = 0; i < LX; i++) {
-    const int r = (wave + 4 * i) * 8 + (lane >> 3);
-    ox[i] = m0 + r < a.m ? (unsigned)(r * (int)a.ldx * ES) + cb : OUTSIDE;
+  for (int i = 0; i < LT; i++) {
+    const int r = (wave + NW * (i < LX ? i : i - LX)) * RPL + lr;
+    if (i < LX) off[i] = m0 + r < a.m ? (unsigned)(r * (int)a.ldx * ES) + cb : OUTSIDE;
+    else off[i] = n0 + r < a.n ? (unsigned)(r * (int)a.ldw * ES) + cb : OUTSIDE;
   }
-#pragma unroll
-  for (int i = 0; i < LW; i++) {
-    const int r = (wave + 4 * i) * 8 + (lane >> 3);
-    ow[i] = n0 + r < a.n ? (unsigned)(r * (int)a.ldw * ES) + cb : OUTSIDE;
-  }
-  auto load = [&](int step, int i) __attribute__((always_inline)) {   // load i of LT: x before w
-    const unsigned s = lds0 + (step & 1) * STAGE, kb = (unsigned)step * 128;
-    const unsigned off = i < LX ? ox[i] : ow[i - LX], to = i < LX ? (wave + 4 * i) * 1024 : BM * 128 + (wave + 4 * (i - LX)) * 1024;
-    dma16(i < LX ? rx : rw, s + to, kb + cb < kbytes ? off : OUTSIDE, kb);   // (past the end of a row: zeros)
+  // load i of LT of `step` into `stage` (x before w); past the end of a row, zeros
+  auto load = [&](int step, int stage, int i) __attribute__((always_inline)) {
+    const unsigned kb = (unsigned)step * RB, to = lds0 + stage * STAGE + (i < LX ? (wave + NW * i) * 1024 : BM * RB + (wave + NW * (i - LX)) * 1024);
+    dma16(i < LX ? rx : rw, to, kb + cb < kbytes ? off[i] : OUTSIDE, kb);
   };
   f32x16 acc[NT][MT];
 #pragma unroll
@@ -274,35 +271,31 @@ __global__ __launch_bounds__(256, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(c
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
   typename S::frag fx[2][MT], fw[2][NT];
-  const int swz = lane & 7;
-  const unsigned char* xrow = smem + (wm * 32 * MT + (lane & 31)) * 128;
-  const unsigned char* wrow = smem + BM * 128 + (wn * 32 * NT + (lane & 31)) * 128;
-  auto read_x = [&](int set, int stage, int ks, int j) __attribute__((always_inline)) { fx[set][j] = S::read(xrow + stage * STAGE + j * 4096, ks, half, swz); };
-  auto read_w = [&](int set, int stage, int ks, int i) __attribute__((always_inline)) { fw[set][i] = S::read(wrow + stage * STAGE + i * 4096, ks, half, swz); };
-
+  const int swz = swizzle(lane & 31);
+  const unsigned char* xrow = smem + (wm * 32 * MT + (lane & 31)) * RB;
+  const unsigned char* wrow = smem + BM * RB + (wn * 32 * NT + (lane & 31)) * RB;
+  auto read = [&](int set, int stage, int ks, int f) __attribute__((always_inline)) {   // operand f: w 0, x 0 .. MT - 1, w 1 ..
+    if (f == 0) fw[set][0] = S::read(wrow + stage * STAGE, ks, half, swz);
+    else if (f <= MT) fx[set][f - 1] = S::read(xrow + stage * STAGE + (f - 1) * 32 * RB, ks, half, swz);
+    else fw[set][f - MT] = S::read(wrow + stage * STAGE + (f - MT) * 32 * RB, ks, half, swz);
+  };
 #pragma unroll
-  for (int i = 0; i < LT; i++) load(0, i);
-  if (nk > 1) {
+  for (int t = 0; t < NST; t++)
 #pragma unroll
-    for (int i = 0; i < LT; i++) load(1, i);
-    if (LT == 16) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-    else if (LT == 12) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-  } else {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  }
-  static_assert(LT == 16 || LT == 12 || LT == 8, "the wait above");
-  __syncthreads();
+    for (int i = 0; i < (NKS > 1 && t == NST - 1 ? LT / 2 : LT); i++) load(t, t, i);
+  wait_loads<(NST - 1) * LT - (NKS > 1 ? LT / 2 : 0)>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 #pragma unroll
-  for (int j = 0; j < MT; j++) read_x(0, 0, 0, j);
-#pragma unroll
-  for (int i = 0; i < NT; i++) read_w(0, 0, 0, i);
+  for (int f = 0; f < MT + NT; f++) read(0, 0, 0, f);
+  int st = 0;
+  // (NKS 1: two steps a turn, so that the operand sets take turns without copies)
 #pragma unroll 1
-  for (int t = 0; t < nk; t++) {
-    const int st = t & 1;
+  for (int t = 0; t < nk; t += NKS == 1 ? 2 : 1) {
 #pragma unroll
-    for (int ks = 0; ks < NKS; ks++) {
-      const int set = ks & 1, last = ks == NKS - 1;
+    for (int u = 0; u < (NKS == 1 ? 2 : NKS); u++) {
+      const int set = u & 1, last = NKS == 1 || u == NKS - 1, step = t + (NKS == 1 ? u : 0);
+      const int nxt = last ? (st + 1 == NST ? 0 : st + 1) : st;
       // a matrix instruction takes 32 cycles (8 bits: 64), so what goes out between two of them costs nothing
 #pragma unroll
       for (int q = 0; q < MT * NT; q++) {
@@ -310,40 +303,59 @@ __global__ __launch_bounds__(256, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(c
         acc[i][j] = S::mfma(fw[set][i], fx[set][j], acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
         if (last && q == 0) {
-          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          wait_loads<(NST - 2) * LT>();
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
         }
-        // operands of the next slice (after the last step: of a stage that is not read any more)
+        // operands of the next slice
         constexpr int RPQ = (MT + NT + MT * NT - 1) / (MT * NT);
 #pragma unroll
-        for (int f = q * RPQ; f < (q + 1) * RPQ && f < MT + NT; f++) {
-          if (f == 0) read_w(set ^ 1, last ? st ^ 1 : st, last ? 0 : ks + 1, 0);
-          else if (f <= MT) read_x(set ^ 1, last ? st ^ 1 : st, last ? 0 : ks + 1, f - 1);
-          else read_w(set ^ 1, last ? st ^ 1 : st, last ? 0 : ks + 1, f - MT);
+        for (int f = q * RPQ; f < (q + 1) * RPQ && f < MT + NT; f++) read(set ^ 1, nxt, last ? 0 : u + 1, f);
+        // loads for NST steps on into the stage that the last barrier freed, evenly over the two slices behind it: a burst of
+        // them holds the wave up (each takes the address unit, which four waves share, 16 cycles)
+        if (NKS > 1) {
+          constexpr int EVERY = 2 * MT * NT / LT;
+          const int p = last ? q : MT * NT + q;
+          if ((last || u == 0) && p % EVERY == 0) load((last ? step : step - 1) + NST, last ? st : st == 0 ? NST - 1 : st - 1, p / EVERY);
+        } else {
+          constexpr int EVERY = MT * NT / LT > 0 ? MT * NT / LT : 1;
+          if (q % EVERY == 0) load(step + NST, st, q / EVERY);
         }
-        // loads for the step after next, one an instruction, from the barrier on
-        if (last && t + 2 < nk && q < LT) load(t + 2, q);
-        if (ks == 0 && t > 0 && t + 1 < nk && MT * NT + q < LT) load(t + 1, MT * NT + q);
         __builtin_amdgcn_sched_barrier(0);
       }
+      st = nxt;
     }
   }
-  static_assert(LT <= 2 * MT * NT, "the loads of a step fit two slices");
+  static_assert(2 * MT * NT % LT == 0 && (NKS > 1 || MT * NT % LT == 0), "the loads of a step fit the slices");
+  wait_loads<0>();   // (zeros for steps past the end may still be on their way)
   // Epilogue: the sums of 32 rows at a time go through LDS (each wave has its own part), after which a lane holds eight
   // neighbours of a row: bias, activation and residual happen there, and rows leave as whole lines.
   __syncthreads();   // (nobody reads the stages any more)
   constexpr int PITCH = 32 * NT * 4 + 16;
-  constexpr int LPR = 4 * NT, RPI = 64 / LPR;   // lanes a row, rows at a time
+  constexpr int LPR = 4 * NT, RPI = 64 / LPR, RI = 32 / RPI;   // lanes a row, rows at a time, times
   unsigned char* ex = smem + wave * 32 * PITCH;
   const int c = (lane % LPR) * 8;
   const int64_t n = n0 + wn * 32 * NT + c, left = a.n - n;
+  const int64_t mw = m0 + wm * 32 * MT + lane / LPR;   // this lane's rows: mw + 32 j + RPI i
+  const bool vec = wide && left >= 8;
   float bias[8], wsc[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     bias[e] = a.bias && e < left ? a.bias[n + e] : 0.f;
     wsc[e] = IN == CRNN_E4M3 && a.w_scale && e < left ? a.w_scale[n + e] : 1.f;
   }
+  // the residual of the next 32 rows (fp32: of these, registers are short) is on its way while these are worked on
+  typedef typename Eight<TO>::t E8;
+  constexpr int AHEAD = sizeof(TO) == 2;
+  E8 res[1 + AHEAD][RI];
+  auto fetch = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < RI; i++) {
+      const int64_t m = mw + 32 * j + RPI * i;
+      if (a.residual && vec && m < a.m) res[j & AHEAD][i] = *(const E8*)((const TO*)a.residual + m * a.ldr + n);
+    }
+  };
+  if (AHEAD) fetch(0);
 #pragma unroll
   for (int j = 0; j < MT; j++) {
 #pragma unroll
@@ -351,20 +363,39 @@ __global__ __launch_bounds__(256, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(c
 #pragma unroll
       for (int g = 0; g < 4; g++)
         *(f32x4*)(ex + (lane & 31) * PITCH + (i * 32 + 8 * g + 4 * half) * 4) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+    if (j + AHEAD < MT) fetch(j + AHEAD);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-    for (int r = lane / LPR; r < 32; r += RPI) {
-      const f32x4 lo = *(const f32x4*)(ex + r * PITCH + c * 4), hi = *(const f32x4*)(ex + r * PITCH + c * 4 + 16);
-      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      const int64_t m = m0 + wm * 32 * MT + j * 32 + r;
-      if (m < a.m && left > 0) {
-        const float sx = IN == CRNN_E4M3 && a.x_scale ? a.x_scale[m] : 1.f;
+    float v[8 * RI];
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = IN == CRNN_E4M3 ? v[e] * sx * wsc[e] + bias[e] : v[e] + bias[e];
-        activate8(v, a.act);
-        put8<TO>(a, m, n, left < 8 ? (int)left : 8, wide, v);
+    for (int i = 0; i < RI; i++) {
+      const int r = lane / LPR + RPI * i;
+      const f32x4 lo = *(const f32x4*)(ex + r * PITCH + c * 4), hi = *(const f32x4*)(ex + r * PITCH + c * 4 + 16);
+      float sx = 1.f;
+      if (IN == CRNN_E4M3 && a.x_scale && mw + 32 * j + RPI * i < a.m) sx = a.x_scale[mw + 32 * j + RPI * i];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float u = e < 4 ? lo[e & 3] : hi[e & 3];
+        v[8 * i + e] = IN == CRNN_E4M3 ? u * sx * wsc[e] + bias[e] : u + bias[e];
       }
+    }
+    activate_all(v, a.act);
+#pragma unroll
+    for (int i = 0; i < RI; i++) {
+      const int64_t m = mw + 32 * j + RPI * i;
+      float u[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) u[e] = v[8 * i + e];
+      if (m >= a.m || left <= 0) continue;
+      if (!vec) {
+        put<TO>(a, m, n, left < 8 ? (int)left : 8, u);
+        continue;
+      }
+      if (a.residual) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) u[e] += (float)res[j & AHEAD][i][e];
+      }
+      store8((TO*)a.y + m * a.ldy + n, u);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
@@ -379,20 +410,20 @@ static bool linear_chunks(const crnn_linear_args& a) {
          (256 * (a.ldx > a.ldw ? a.ldx : a.ldw) + a.k) * es < 0x7FFFFFFF;
 }
 
-template <int IN, int OUT, int MT, int NT>
+template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST>
 static void linear_tile(const crnn_linear_args& a, hipStream_t s) {
   const int64_t eo = OUT == CRNN_FP32 ? 4 : 2;
   auto chunks = [&](const void* p, int64_t ld) { return (((uintptr_t)p | (uintptr_t)(ld * eo)) & 15) == 0; };
   const int wide = chunks(a.y, a.ldy) && (!a.residual || chunks(a.residual, a.ldr));
-  const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 64 * NT - 1) / (64 * NT));
-  hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), 0, s, a, wide);
+  const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 32 * WN * NT - 1) / (32 * WN * NT));
+  hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT, WN, RB, NST>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(128 * WN), 0, s, a, wide);
 }
 template <int IN, int OUT>
 static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
   if ((a.m + 63) / 64 * ((a.n + 63) / 64) >= 1 << 23) return false;   // (a launch has fewer than 2^32 threads)
   const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
-  if (big >= 192) linear_tile<IN, OUT, 4, 4>(a, s);
-  else linear_tile<IN, OUT, 2, 2>(a, s);
+  if (big >= 192) linear_tile<IN, OUT, 4, 2, 4, 128, 2>(a, s);
+  else linear_tile<IN, OUT, 2, 2, 2, 128, 2>(a, s);
   return true;
 }
 
@@ -723,8 +754,8 @@ __global__ __launch_bounds__(256, 2) void attention_any_kernel(const crnn_cross_
 // (v_mfma_f32_32x32x16_bf16): a lane then holds one query row in both results, so maximum, sum and rescaling are per lane, and
 // the exponentials are the second product's operand as they stand, because its sum may run over the keys in any order: register
 // r of S^T is key (r & 3) + 8 (r >> 2) + 4 (lane >> 5), and ds_read_tr16_b64 takes V's columns for four such keys at a time.
-// K and V tiles go straight to LDS, two stages; 16-byte chunk c of row j sits at chunk c ^ swizzle(j), which spreads the eight
-// rows (K) or the four half rows (V) that are read at once over all banks.  Keys that are left out are never loaded: their
+// K and V tiles go straight to LDS, two stages; 16-byte chunk c of row j sits at chunk c ^ swizzle(j), which spreads what is
+// read at once -- 16 rows of K, 64 bytes of four rows of V -- over the 256 bytes that LDS serves in a cycle.  Keys that are left out are never loaded: their
 // offset lies outside the resource, LDS gets zeros, and their score is -inf.
 // With nsplit > 1 workgroups share the keys of one row block and leave (O, M, L) for attention_join_kernel.
 struct AttnPlan {
@@ -773,8 +804,8 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const c
       q[kk] = __builtin_bit_cast(bf16x8, u);
     }
   }
-  auto swz_k = [](int r) { return NCH % 8 == 0 ? r & 7 : (r >> 1) & 3; };
-  auto swz_v = [](int r) { return NCH % 8 == 0 ? 2 * (r & 3) : 2 * ((r >> 1) & 1); };
+  auto swz_k = [](int r) { return NCH == 16 ? r & 15 : NCH == 8 ? (r >> 1) & 7 : (r >> 2) & 3; };
+  auto swz_v = [](int r) { return NCH == 16 ? 4 * (r & 3) : NCH == 8 ? 2 * (r & 2) : 0; };
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem + kw * 4 * TILE;
   const unsigned char* base = smem + kw * 4 * TILE;
 
