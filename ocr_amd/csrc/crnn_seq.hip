@@ -207,6 +207,17 @@ template <> struct Slice<CRNN_E4M3> {
   static __device__ __forceinline__ f32x16 mfma(frag w, frag x, f32x16 c) { return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, 0, 0, 0, 0); }
 };
 
+template <> struct Slice<CRNN_FP32> {   // one 16-byte chunk a lane: four v_mfma_f32_32x32x2_f32, each with one value of both halves
+  static constexpr int KB = 32;
+  typedef f32x4 frag;
+  static __device__ __forceinline__ frag read(const unsigned char* row, int ks, int half, int swz) { return *(const f32x4*)(row + (((2 * ks + half) ^ swz) << 4)); }
+  static __device__ __forceinline__ f32x16 mfma(frag w, frag x, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(w[i], x[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
 // Up to eight values of a row of y, one by one: residual, rounding, store.
 template <typename TO>
 __device__ __forceinline__ void put(const crnn_linear_args& a, int64_t m, int64_t n, int count, const float (&v)[8]) {
@@ -226,7 +237,7 @@ template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST>
 __global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a, int wide) {
   typedef Slice<IN> S;
   typedef typename TypeOf<OUT>::t TO;
-  constexpr int ES = IN == CRNN_BF16 ? 2 : 1, NKS = RB / S::KB, RPL = 1024 / RB;   // slices of a step, rows of a load
+  constexpr int ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1, NKS = RB / S::KB, RPL = 1024 / RB;   // slices of a step, rows of a load
   constexpr int NW = 2 * WN, BM = 64 * MT, BN = 32 * WN * NT, STAGE = (BM + BN) * RB;
   constexpr int LX = BM / (RPL * NW), LT = (BM + BN) / (RPL * NW);   // dma16 instructions of a wave and step: of x, all
   __shared__ __attribute__((aligned(1024))) unsigned char smem[NST * STAGE];
@@ -283,7 +294,7 @@ __global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_ker
   for (int t = 0; t < NST; t++)
 #pragma unroll
     for (int i = 0; i < (NKS > 1 && t == NST - 1 ? LT / 2 : LT); i++) load(t, t, i);
-  wait_loads<(NST - 1) * LT - (NKS > 1 ? LT / 2 : 0)>();
+  wait_loads<(NST - 1) * LT - (NKS > 1 ? LT - LT / 2 : 0)>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
@@ -313,20 +324,17 @@ __global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_ker
         for (int f = q * RPQ; f < (q + 1) * RPQ && f < MT + NT; f++) read(set ^ 1, nxt, last ? 0 : u + 1, f);
         // loads for NST steps on into the stage that the last barrier freed, evenly over the two slices behind it: a burst of
         // them holds the wave up (each takes the address unit, which four waves share, 16 cycles)
-        if (NKS > 1) {
-          constexpr int EVERY = 2 * MT * NT / LT;
-          const int p = last ? q : MT * NT + q;
-          if ((last || u == 0) && p % EVERY == 0) load((last ? step : step - 1) + NST, last ? st : st == 0 ? NST - 1 : st - 1, p / EVERY);
-        } else {
-          constexpr int EVERY = MT * NT / LT > 0 ? MT * NT / LT : 1;
-          if (q % EVERY == 0) load(step + NST, st, q / EVERY);
+        constexpr int SLOTS = NKS > 1 ? 2 * MT * NT : MT * NT;
+        const int p = last ? q : MT * NT + q;
+        if (last || (NKS > 1 && u == 0)) {
+#pragma unroll
+          for (int l = p * LT / SLOTS; l < (p + 1) * LT / SLOTS; l++) load((last ? step : step - 1) + NST, last ? st : st == 0 ? NST - 1 : st - 1, l);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
       st = nxt;
     }
   }
-  static_assert(2 * MT * NT % LT == 0 && (NKS > 1 || MT * NT % LT == 0), "the loads of a step fit the slices");
   wait_loads<0>();   // (zeros for steps past the end may still be on their way)
   // Epilogue: the sums of 32 rows at a time go through LDS (each wave has its own part), after which a lane holds eight
   // neighbours of a row: bias, activation and residual happen there, and rows leave as whole lines.
@@ -402,12 +410,92 @@ __global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_ker
   }
 }
 
+// ---------------------------------------------------------------------------
+// linear, few rows (at most 64) of whole 16-byte chunks: 32 columns of y per workgroup, whose KW waves take 128 bytes of k of
+// every row of w in turn and add up through LDS in a fixed order.  Bound by reading w, or by the way of the first bytes: no
+// LDS on the way in, every lane loads its operands as they lie (the products may be added in any order, so a lane's half of a
+// block is 64 neighbouring bytes), the next block's while this one is multiplied.  x is the first operand: lanes hold
+// neighbouring columns.
+// ---------------------------------------------------------------------------
+template <int IN, int OUT, int MT, int KW>
+__global__ __launch_bounds__(64 * KW, 2) void linear_rows_kernel(const crnn_linear_args a) {
+  typedef typename TypeOf<OUT>::t TO;
+  typedef Slice<IN> S;
+  constexpr int ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1;
+  __shared__ float part[KW][MT * 16][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int64_t n0 = (int64_t)blockIdx.x * 32;
+  const unsigned kbytes = (unsigned)a.k * ES;
+  const int nb = (int)((kbytes + 127) / 128);
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)a.x, 0, 0x7FFFFFFF, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.w + n0 * a.ldw * ES), 0, 0x7FFFFFFF, 0x00020000);
+  const unsigned ow = n0 + (lane & 31) < a.n ? (unsigned)((lane & 31) * (int)a.ldw * ES) + half * 64u : OUTSIDE;
+  unsigned ox[MT];
+#pragma unroll
+  for (int j = 0; j < MT; j++) ox[j] = 32 * j + (lane & 31) < a.m ? (unsigned)((32 * j + (lane & 31)) * (int)a.ldx * ES) + half * 64u : OUTSIDE;
+  f32x16 acc[MT];
+#pragma unroll
+  for (int j = 0; j < MT; j++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[j][r] = 0.f;
+  i32x4 w[2][4], x[2][MT][4];
+  auto load = [&](int set, int blk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const unsigned kb = (unsigned)blk * 128 + c * 16;
+      const bool in = kb + half * 64u < kbytes;   // (a block past the end: zeros)
+      w[set][c] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? ow + kb : OUTSIDE, 0, 0);
+#pragma unroll
+      for (int j = 0; j < MT; j++) x[set][j][c] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? ox[j] + kb : OUTSIDE, 0, 0);
+    }
+  };
+  auto multiply = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < MT; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c += IN == CRNN_E4M3 ? 2 : 1) {
+        if constexpr (IN == CRNN_E4M3) {
+          const i32x4 x0 = x[set][j][c], x1 = x[set][j][c + 1], w0 = w[set][c], w1 = w[set][c + 1];
+          acc[j] = S::mfma(i32x8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]}, i32x8{w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]}, acc[j]);
+        } else {
+          acc[j] = S::mfma(__builtin_bit_cast(typename S::frag, x[set][j][c]), __builtin_bit_cast(typename S::frag, w[set][c]), acc[j]);
+        }
+      }
+  };
+  load(0, wave);
+  for (int blk = wave; blk < nb; blk += 2 * KW) {
+    load(1, blk + KW);
+    multiply(0);
+    load(0, blk + 2 * KW);
+    multiply(1);
+  }
+#pragma unroll
+  for (int j = 0; j < MT; j++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) part[wave][j * 16 + r][lane] = acc[j][r];
+  __syncthreads();
+  const int64_t n = n0 + (lane & 31);
+  if (n >= a.n) return;
+  const float bias = a.bias ? a.bias[n] : 0.f, wsc = IN == CRNN_E4M3 && a.w_scale ? a.w_scale[n] : 1.f;
+  for (int i = wave; i < MT * 16; i += KW) {
+    const int m = (i >> 4) * 32 + acc_row(i & 15, lane);
+    if (m >= a.m) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int s = 0; s < KW; s++) v += part[s][i][lane];
+    if (IN == CRNN_E4M3) v = v * (a.x_scale ? a.x_scale[m] : 1.f) * wsc;
+    v = activate(v + bias, a.act);
+    if (a.residual) v += (float)((const TO*)a.residual)[m * a.ldr + n];
+    ((TO*)a.y)[m * a.ldy + n] = (TO)v;
+  }
+}
+
 // Rows of whole 16-byte chunks, and offsets within a tile below 2^31 bytes.
 static bool linear_chunks(const crnn_linear_args& a) {
-  const int64_t es = a.in_type == CRNN_BF16 ? 2 : 1, c = 16 / es;
-  if (a.in_type == CRNN_FP32 || (a.in_type == CRNN_E4M3 && a.out_type == CRNN_FP32)) return false;
+  const int64_t es = a.in_type == CRNN_FP32 ? 4 : a.in_type == CRNN_BF16 ? 2 : 1, c = 16 / es;
+  if (a.in_type == CRNN_E4M3 && a.out_type == CRNN_FP32) return false;
   return a.k % c == 0 && a.ldx % c == 0 && a.ldw % c == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 &&
-         (256 * (a.ldx > a.ldw ? a.ldx : a.ldw) + a.k) * es < 0x7FFFFFFF;
+         (256 * (a.ldx > a.ldw ? a.ldx : a.ldw) + a.k) * es < 0x7FFFF000;
 }
 
 template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST>
@@ -420,17 +508,39 @@ static void linear_tile(const crnn_linear_args& a, hipStream_t s) {
 }
 template <int IN, int OUT>
 static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
-  if ((a.m + 63) / 64 * ((a.n + 63) / 64) >= 1 << 23) return false;   // (a launch has fewer than 2^32 threads)
-  const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
-  if (big >= 192) linear_tile<IN, OUT, 4, 2, 4, 128, 2>(a, s);
-  else linear_tile<IN, OUT, 2, 2, 2, 128, 2>(a, s);
+  if ((a.m + 63) / 64 * ((a.n + 63) / 64) >= 1 << 22) return false;   // (a launch has fewer than 2^32 threads)
+  // Tiles come in rounds of what the 256 CUs hold; a round takes its tile's size (256 x 256: 4), 128 x 128 ones two a CU with
+  // less use of what is loaded.  18176 x 512 x 2048: 256 rows 54 us, 192 rows 50, 128 x 128 59; 16384 x 4096 x 4096: 455, 488, 556.
+  auto rounds = [&](int bm, int bn, int at_once) { return (double)(((a.m + bm - 1) / bm * ((a.n + bn - 1) / bn) + at_once - 1) / at_once); };
+  const double c4 = 4.0 * rounds(256, 256, 256), c3 = 3.0 * rounds(192, 256, 256), c2 = 2.4 * rounds(128, 128, 512);
+  const int64_t small = ((a.m + 127) / 128) * ((a.n + 127) / 128);
+  if constexpr (IN != CRNN_FP32) {
+    if (c4 <= c3 && c4 <= c2) return linear_tile<IN, OUT, 4, 2, 4, 128, 2>(a, s), true;
+    if (c3 <= c2) return linear_tile<IN, OUT, 3, 2, 4, 128, 2>(a, s), true;
+  }
+  if (small >= 256) linear_tile<IN, OUT, 2, 2, 2, 128, 2>(a, s);
+  else linear_tile<IN, OUT, 1, 1, 2, 128, 4>(a, s);
   return true;
+}
+
+template <int IN, int OUT, int MT>
+static void linear_rows(const crnn_linear_args& a, hipStream_t s) {
+  constexpr int ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1;
+  const dim3 g((unsigned)((a.n + 31) / 32));
+  if (a.k * ES <= 1024) hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, MT, 4>), g, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, MT, 8>), g, dim3(512), 0, s, a);
 }
 
 template <int IN, int OUT>
 static void linear_of(const crnn_linear_args& a, hipStream_t s) {
-  if constexpr (IN == CRNN_BF16 || (IN == CRNN_E4M3 && OUT == CRNN_BF16)) {
-    if (linear_chunks(a) && linear_tiles<IN, OUT>(a, s)) return;
+  if constexpr (IN != CRNN_E4M3 || OUT == CRNN_BF16) {
+    if (linear_chunks(a)) {
+      if (a.m <= 64 && a.n < 1 << 27) {
+        a.m <= 32 ? linear_rows<IN, OUT, 1>(a, s) : linear_rows<IN, OUT, 2>(a, s);
+        return;
+      }
+      if (linear_tiles<IN, OUT>(a, s)) return;
+    }
   }
   hipLaunchKernelGGL((linear_any_kernel<IN, OUT>), grid_for((a.m + 63) / 64 * ((a.n + 63) / 64)), dim3(256), 0, s, a);
 }
