@@ -200,13 +200,13 @@ def lib():
     L.crnn_channel_scales.restype = C.c_int
     L.crnn_channel_scales.argtypes = [vp, i32, C.POINTER(C.c_float), i32]
     L.crnn_linear.restype = C.c_int
-    L.crnn_linear.argtypes = [vp, C.POINTER(LinearArgs), vp]
+    L.crnn_linear.argtypes = [vp, C.c_void_p, vp]   # LinearArgs, by reference or as bytes
     L.crnn_rms_norm.restype = C.c_int
-    L.crnn_rms_norm.argtypes = [vp, C.POINTER(RmsNormArgs), vp]
+    L.crnn_rms_norm.argtypes = [vp, C.c_void_p, vp]   # RmsNormArgs, by reference or as bytes
     L.crnn_cross_attention.restype = C.c_int
-    L.crnn_cross_attention.argtypes = [vp, C.POINTER(CrossAttentionArgs), vp]
+    L.crnn_cross_attention.argtypes = [vp, C.c_void_p, vp]   # CrossAttentionArgs, by reference or as bytes
     L.crnn_cross_attention_workspace.restype = C.c_int64
-    L.crnn_cross_attention_workspace.argtypes = [vp, C.POINTER(CrossAttentionArgs)]
+    L.crnn_cross_attention_workspace.argtypes = [vp, C.c_void_p]
     L.crnn_states_device.restype = C.c_int
     L.crnn_states_device.argtypes = [vp, vp, i32, i32, vp, vp, vp, vp]
     _lib = L

@@ -859,6 +859,17 @@ __global__ __launch_bounds__(256, 2) void attention_any_kernel(const crnn_cross_
   }
 }
 
+// Where split s of nsplit leaves row r of all rows (batch, key head, row): D unnormalised values, then (M, L) behind all of them.
+constexpr int MAX_SPLIT = 64;
+struct SplitRow {
+  float *o, *ml;
+  __device__ __forceinline__ SplitRow(const crnn_cross_attention_args& a, int nsplit, int s, int64_t r) {
+    const int64_t all = a.batch * a.heads * a.q_len;
+    o = (float*)a.workspace + (s * all + r) * a.head_dim;
+    ml = (float*)a.workspace + nsplit * all * a.head_dim + (s * all + r) * 2;
+  }
+};
+
 // bf16, head_dim and strides in whole 16-byte chunks.  Four waves (or one): RW of them side by side over 32 rows each, KW of
 // them over different tiles of KT keys; head_dim padded to DP.  Both products run transposed, S^T = K Q^T and O^T = V^T P^T
 // (v_mfma_f32_32x32x16_bf16): a lane then holds one query row in both results, so maximum, sum and rescaling are per lane, and
@@ -868,10 +879,6 @@ __global__ __launch_bounds__(256, 2) void attention_any_kernel(const crnn_cross_
 // read at once -- 16 rows of K, 64 bytes of four rows of V -- over the 256 bytes that LDS serves in a cycle.  Keys that are left out are never loaded: their
 // offset lies outside the resource, LDS gets zeros, and their score is -inf.
 // With nsplit > 1 workgroups share the keys of one row block and leave (O, M, L) for attention_join_kernel.
-struct AttnPlan {
-  int rw, kw, nsplit;
-};
-
 template <int DP, int RW, int KW, int KT>
 __global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const crnn_cross_attention_args a, int nsplit) {
   constexpr int NCH = DP / 8, ROWB = DP * 2, TILE = KT * ROWB, NW = RW * KW;   // chunks of a row, bytes of a row and of a tile
@@ -1069,16 +1076,15 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const c
   }
   if (!live) return;
   if (nsplit > 1) {
-    // [split][row of all blocks][D values, M, L] fp32
-    float* ws = (float*)a.workspace + ((int64_t)sp * (a.batch * a.kv_heads * rows) + bg * rows + row) * (D + 2);
+    const SplitRow w(a, nsplit, sp, bg * rows + row);
 #pragma unroll
     for (int i = 0; i < DP / 32; i++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int d = i * 32 + acc_row(r, lane);
-        if (d < D) ws[d] = o[i][r];
+      for (int r = 0; r < 16; r += 4) {
+        const int d = i * 32 + acc_row(r, lane);   // four neighbours; head_dim is a multiple of 8
+        if (d < D) *(f32x4*)(w.o + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
       }
-    if (half == 0) ws[D] = Me, ws[D + 1] = L;
+    if (half == 0) w.ml[0] = Me, w.ml[1] = L;
     return;
   }
   __bf16* out = (__bf16*)a.out + b * a.out_stride[0] + row / G * a.out_stride[1] + (g * G + row % G) * a.out_stride[2];
@@ -1092,54 +1098,303 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const c
     }
 }
 
-// out = sum_s O_s 2^(M_s - M) / sum_s L_s 2^(M_s - M), a thread per value of out
-template <int TYPE>
+// A few rows (at most four) per key head: no matrix instructions, no LDS on the way in.  LPK lanes share a key (16 bytes of it
+// each), so an instruction loads 64 / LPK keys; a wave takes chunks of U such groups, the next chunk's loads on their way while
+// this one is worked on.  Every group of lanes keeps a maximum, a sum and a result over its own keys; they are joined at the
+// end, lanes by exchange, the KW waves through LDS, nsplit workgroups by attention_join_kernel.  Keys that are left out are not
+// loaded.  Bound by reading the keys.
+template <int TYPE, int LPK, int U, int R, int KW>
+__global__ __launch_bounds__(64 * KW, 2) void attention_few_kernel(const crnn_cross_attention_args a, int nsplit) {
+  typedef typename TypeOf<TYPE>::t T;
+  constexpr int ES = sizeof(T), EPC = 16 / ES, KPI = 64 / LPK, KEYS = U * KPI;
+  __shared__ float part[KW][R][LPK * EPC + 2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane % LPK, grp = lane / LPK;
+  const int G = a.heads / a.kv_heads, D = a.head_dim, rows = (int)a.q_len * G;
+  const int64_t total = a.batch * a.kv_heads * nsplit, per = (total + 7) / 8, blk = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (blk >= total || (blockIdx.x >> 3) >= per) return;
+  const int sp = (int)(blk % nsplit);
+  const int64_t bg = blk / nsplit, b = bg / a.kv_heads, g = bg % a.kv_heads;
+  const int len = a.lengths ? max(0, (int)min((int64_t)a.lengths[b], a.kv_len)) : (int)a.kv_len;
+  const int steps_all = (len + KEYS * KW - 1) / (KEYS * KW), steps_per = (steps_all + nsplit - 1) / nsplit;
+  const int step0 = min(sp * steps_per, steps_all), steps = min(steps_per, steps_all - step0);
+  const T* kp = (const T*)a.k + b * a.k_stride[0] + g * a.k_stride[2];
+  const T* vp = (const T*)a.v + b * a.v_stride[0] + g * a.v_stride[2];
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
+  const bool din = c * EPC < D;
+  // keys of a chunk that count, one bit each
+  auto mask_byte = [&](int step) __attribute__((always_inline)) -> int {
+    const int j = (step * KW + wave) * KEYS + lane;
+    return mask && lane < KEYS && j < len ? mask[j] : 0;
+  };
+  auto bits_of = [&](int step, int mb) __attribute__((always_inline)) -> unsigned long long {
+    const int left = len - (step * KW + wave) * KEYS;
+    unsigned long long w = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+    if (KEYS < 64) w &= (1ull << (KEYS & 63)) - 1;
+    return mask ? w & __ballot(mb != 0) : w;
+  };
+  i32x4 kr[2][U], vr[2][U];
+  auto load = [&](int set, int step, unsigned long long w) __attribute__((always_inline)) {
+    const int64_t j0 = (int64_t)(step * KW + wave) * KEYS;
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + j0 * a.k_stride[1]), 0, 0x7FFFFFFF, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + j0 * a.v_stride[1]), 0, 0x7FFFFFFF, 0x00020000);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int r = u * KPI + grp;
+      const bool in = din && ((w >> r) & 1);
+      kr[set][u] = __builtin_amdgcn_raw_buffer_load_b128(rk, in ? (unsigned)(r * (int)a.k_stride[1] * ES) + c * 16u : OUTSIDE, 0, 0);
+      vr[set][u] = __builtin_amdgcn_raw_buffer_load_b128(rv, in ? (unsigned)(r * (int)a.v_stride[1] * ES) + c * 16u : OUTSIDE, 0, 0);
+    }
+  };
+  auto widen = [](i32x4 x, float (&v)[EPC]) __attribute__((always_inline)) {
+    if constexpr (ES == 4) {
+      const f32x4 f = __builtin_bit_cast(f32x4, x);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = f[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float((unsigned)x[i] << 16), v[2 * i + 1] = __uint_as_float((unsigned)x[i] & 0xFFFF0000u);
+    }
+  };
+  unsigned long long w = 0, wn = 0;
+  if (steps > 0) {
+    const int mb1 = steps > 1 ? mask_byte(step0 + 1) : 0;
+    w = bits_of(step0, mask_byte(step0));
+    load(0, step0, w);
+    if (steps > 1) wn = bits_of(step0 + 1, mb1);
+  }
+  // the queries, with scale and log2 e in them (exp(x) = 2^(x log2 e))
+  float q[R][EPC];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const bool in = r < rows && din;
+    i32x4 x = {0, 0, 0, 0};
+    if (in) x = *(const i32x4*)((const T*)a.q + b * a.q_stride[0] + r / G * a.q_stride[1] + (g * G + r % G) * a.q_stride[2] + c * EPC);
+    widen(x, q[r]);
+#pragma unroll
+    for (int i = 0; i < EPC; i++) q[r][i] *= a.scale * 1.4426950408889634f;
+  }
+  float M[R], L[R], o[R][EPC];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    M[r] = -INFINITY, L[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPC; i++) o[r][i] = 0.f;
+  }
+  auto work = [&](int set, unsigned long long bits) __attribute__((always_inline)) {
+    if (bits == 0) return;
+    float s[R][U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float k[EPC];
+      widen(kr[set][u], k);
+      const bool in = (bits >> (u * KPI + grp)) & 1;
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < EPC; i++) t = fmaf(q[r][i], k[i], t);
+#pragma unroll
+        for (int f = 1; f < LPK; f <<= 1) t += __shfl_xor(t, f);
+        s[r][u] = in ? t : -INFINITY;
+      }
+    }
+    float al[R], Ms[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      float m = M[r];
+#pragma unroll
+      for (int u = 0; u < U; u++) m = fmaxf(m, s[r][u]);
+      Ms[r] = m == -INFINITY ? 0.f : m;
+      al[r] = __builtin_amdgcn_exp2f(M[r] - Ms[r]);
+      M[r] = m;
+      L[r] *= al[r];
+#pragma unroll
+      for (int i = 0; i < EPC; i++) o[r][i] *= al[r];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float v[EPC];
+      widen(vr[set][u], v);
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float p = __builtin_amdgcn_exp2f(s[r][u] - Ms[r]);
+        L[r] += p;
+#pragma unroll
+        for (int i = 0; i < EPC; i++) o[r][i] = fmaf(p, v[i], o[r][i]);
+      }
+    }
+  };
+  auto turn = [&](int set, int it) __attribute__((always_inline)) {
+    if (it >= steps) return;
+    int mb = 0;
+    if (it + 2 < steps) mb = mask_byte(step0 + it + 2);
+    if (it + 1 < steps) load(set ^ 1, step0 + it + 1, wn);
+    work(set, w);
+    w = wn;
+    if (it + 2 < steps) wn = bits_of(step0 + it + 2, mb);
+  };
+  for (int it = 0; it < steps; it += 2) {
+    turn(0, it);
+    turn(1, it + 1);
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+#pragma unroll
+    for (int f = LPK; f < 64; f <<= 1) {
+      const float m2 = __shfl_xor(M[r], f), l2 = __shfl_xor(L[r], f), m = fmaxf(M[r], m2), ms = m == -INFINITY ? 0.f : m;
+      const float a1 = __builtin_amdgcn_exp2f(M[r] - ms), a2 = __builtin_amdgcn_exp2f(m2 - ms);
+      L[r] = L[r] * a1 + l2 * a2;
+#pragma unroll
+      for (int i = 0; i < EPC; i++) o[r][i] = o[r][i] * a1 + __shfl_xor(o[r][i], f) * a2;
+      M[r] = m;
+    }
+  }
+  if constexpr (KW > 1) {
+    if (grp == 0) {
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+#pragma unroll
+        for (int i = 0; i < EPC; i++) part[wave][r][c * EPC + i] = o[r][i];
+        if (c == 0) part[wave][r][LPK * EPC] = M[r], part[wave][r][LPK * EPC + 1] = L[r];
+      }
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int k = 1; k < KW; k++) {
+        const float m2 = part[k][r][LPK * EPC], l2 = part[k][r][LPK * EPC + 1], m = fmaxf(M[r], m2), ms = m == -INFINITY ? 0.f : m;
+        const float a1 = __builtin_amdgcn_exp2f(M[r] - ms), a2 = __builtin_amdgcn_exp2f(m2 - ms);
+        L[r] = L[r] * a1 + l2 * a2;
+#pragma unroll
+        for (int i = 0; i < EPC; i++) o[r][i] = o[r][i] * a1 + part[k][r][c * EPC + i] * a2;
+        M[r] = m;
+      }
+  }
+  if (grp != 0 || !din) return;
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    if (r >= rows) break;
+    if (nsplit > 1) {
+      const SplitRow w(a, nsplit, sp, bg * rows + r);
+#pragma unroll
+      for (int i = 0; i < EPC; i += 4) *(f32x4*)(w.o + c * EPC + i) = f32x4{o[r][i], o[r][i + 1], o[r][i + 2], o[r][i + 3]};
+      if (c == 0) w.ml[0] = M[r], w.ml[1] = L[r];
+    } else {
+      T* out = (T*)a.out + b * a.out_stride[0] + r / G * a.out_stride[1] + (g * G + r % G) * a.out_stride[2] + c * EPC;
+      const float il = L[r] == 0.f ? 0.f : 1.f / L[r];
+#pragma unroll
+      for (int i = 0; i < EPC; i++) out[i] = (T)(o[r][i] * il);
+    }
+  }
+}
+
+// out = sum_s O_s 2^(M_s - M) / sum_s L_s 2^(M_s - M): a workgroup per row, LP lanes with four values each per split, 256 / LP
+// splits side by side, so that everything is asked for at once; the groups meet in LDS.
+template <int TYPE, int LP>
 __global__ __launch_bounds__(256) void attention_join_kernel(const crnn_cross_attention_args a, int nsplit) {
   typedef typename TypeOf<TYPE>::t T;
-  const int G = a.heads / a.kv_heads, D = a.head_dim;
-  const int64_t rows = a.q_len * G, all = a.batch * a.kv_heads * rows, total = all * D;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / D, bg = r / rows, row = r - bg * rows;
-    const int d = (int)(i - r * D);
-    const float* ws = (const float*)a.workspace + r * (D + 2);
-    float M = -INFINITY, L = 0.f, o = 0.f;
-    for (int s = 0; s < nsplit; s++) M = fmaxf(M, ws[s * all * (D + 2) + D]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-    for (int s = 0; s < nsplit; s++) {
-      const float* w = ws + s * all * (D + 2);
-      const float e = exp2f(w[D] - Ms);
-      L += w[D + 1] * e;
-      o += w[d] * e;
+  constexpr int GR = 256 / LP, PER = MAX_SPLIT / GR;
+  __shared__ float po[GR][LP * 4], pm[GR][2];
+  const int G = a.heads / a.kv_heads, D = a.head_dim, tid = threadIdx.x, c = tid % LP, grp = tid / LP;
+  const int64_t rows = a.q_len * G, all = a.batch * a.kv_heads * rows;
+  for (int64_t r = blockIdx.x; r < all; r += gridDim.x) {
+    f32x4 o[PER];
+    float m[PER], l[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int s = grp + i * GR;
+      const SplitRow w(a, nsplit, s, r);
+      o[i] = f32x4{0.f, 0.f, 0.f, 0.f}, m[i] = -INFINITY, l[i] = 0.f;
+      if (s < nsplit) {
+        m[i] = w.ml[0], l[i] = w.ml[1];
+        if (4 * c < D) o[i] = *(const f32x4*)(w.o + 4 * c);
+      }
     }
-    T* out = (T*)a.out + bg / a.kv_heads * a.out_stride[0] + row / G * a.out_stride[1] + (bg % a.kv_heads * G + row % G) * a.out_stride[2];
-    out[d] = (T)(L == 0.f ? 0.f : o / L);
+    float M = m[0];
+#pragma unroll
+    for (int i = 1; i < PER; i++) M = fmaxf(M, m[i]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const float e = __builtin_amdgcn_exp2f(m[i] - Ms);
+      L = fmaf(l[i], e, L);
+#pragma unroll
+      for (int k = 0; k < 4; k++) v[k] = fmaf(o[i][k], e, v[k]);
+    }
+    *(f32x4*)&po[grp][4 * c] = v;
+    if (c == 0) pm[grp][0] = M, pm[grp][1] = L;
+    __syncthreads();
+    if (tid < D) {
+      M = pm[0][0];
+#pragma unroll
+      for (int i = 1; i < GR; i++) M = fmaxf(M, pm[i][0]);
+      const float Mz = M == -INFINITY ? 0.f : M;
+      float x = 0.f;
+      L = 0.f;
+#pragma unroll
+      for (int i = 0; i < GR; i++) {
+        const float e = __builtin_amdgcn_exp2f(pm[i][0] - Mz);
+        L = fmaf(pm[i][1], e, L);
+        x = fmaf(po[i][tid], e, x);
+      }
+      const int64_t bg = r / rows, row = r - bg * rows;
+      T* out = (T*)a.out + bg / a.kv_heads * a.out_stride[0] + row / G * a.out_stride[1] + (bg % a.kv_heads * G + row % G) * a.out_stride[2];
+      out[tid] = (T)(L == 0.f ? 0.f : x / L);
+    }
+    __syncthreads();
   }
 }
 
 static bool attention_chunks(const crnn_cross_attention_args& a) {   // (sizes, type and strides only)
-  if (a.type != CRNN_BF16 || a.head_dim % 8 != 0 || a.kv_len == 0) return false;
+  const int c = a.type == CRNN_BF16 ? 8 : 4;
+  if (a.head_dim % c != 0 || a.kv_len == 0) return false;
   for (int i = 0; i < 3; i++)
-    if (a.q_stride[i] % 8 != 0 || a.k_stride[i] % 8 != 0 || a.v_stride[i] % 8 != 0) return false;
-  return a.k_stride[1] < (1 << 23) && a.v_stride[1] < (1 << 23);   // a tile's offsets stay below 2^31 bytes
+    if (a.q_stride[i] % c != 0 || a.k_stride[i] % c != 0 || a.v_stride[i] % c != 0) return false;
+  return a.k_stride[1] < (1 << 22) && a.v_stride[1] < (1 << 22);   // offsets within 64 keys stay below 2^31 bytes
 }
 static bool attention_aligned(const crnn_cross_attention_args& a) { return (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0; }
 
+// How the work is cut: `rw` waves side by side over 32 rows each, or 0 for attention_few_kernel; `kw` waves over the keys;
+// nsplit workgroups over the keys where there are too few row blocks to fill the chip (512 workgroups are two per CU).
+struct AttnPlan {
+  int rw, kw, nsplit;
+};
 static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
   const int64_t rows = a.q_len * (a.heads / a.kv_heads), bg = a.batch * a.kv_heads;
   AttnPlan p;
-  p.rw = rows > 64 ? 4 : rows > 32 ? 2 : 1;
-  p.kw = 4 / p.rw;
-  const int kt = p.rw == 4 ? 64 : 32;
-  if (p.rw == 1 && a.kv_len <= 4 * kt && bg >= 1024) p.kw = 1;   // few keys, many heads: a wave a head, nothing to join
-  const int64_t blocks = bg * ((rows + 32 * p.rw - 1) / (32 * p.rw)), steps = (a.kv_len + kt * p.kw - 1) / (kt * p.kw);
+  int64_t blocks, keys;   // row blocks; keys of a workgroup's step
+  if (rows <= 4) {
+    p.rw = 0;
+    p.kw = a.kv_len <= 128 && bg >= 1024 ? 1 : 4;   // few keys, many heads: a wave a head, nothing to join
+    blocks = bg;
+    keys = 64 * p.kw;
+  } else {
+    p.rw = rows > 64 ? 4 : rows > 32 ? 2 : 1;
+    p.kw = 4 / p.rw;
+    const int kt = p.rw == 4 ? 64 : 32;
+    if (p.rw == 1 && a.kv_len <= 4 * kt && bg >= 1024) p.kw = 1;
+    blocks = bg * ((rows + 32 * p.rw - 1) / (32 * p.rw));
+    keys = kt * p.kw;
+  }
+  const int64_t steps = (a.kv_len + keys - 1) / keys;
   int64_t ns = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
-  ns = ns < steps / 2 ? ns : steps / 2;                            // at least two steps each
-  p.nsplit = (int)(ns < 1 ? 1 : ns > 256 ? 256 : ns);
+  if (p.rw != 0 && ns > steps / 2) ns = steps / 2;   // at least two steps each
+  if (ns > steps) ns = steps;
+  p.nsplit = (int)(ns < 1 ? 1 : ns > MAX_SPLIT ? MAX_SPLIT : ns);
   return p;
+}
+static bool attention_any(const crnn_cross_attention_args& a) {   // shapes that only attention_any_kernel takes
+  if (!attention_chunks(a)) return true;
+  return a.type == CRNN_FP32 && a.q_len * (a.heads / a.kv_heads) > 4;
 }
 
 int64_t cross_attention_workspace(const crnn_cross_attention_args& a) {
-  if (!attention_chunks(a)) return 0;
+  if (attention_any(a)) return 0;
   const AttnPlan p = attention_plan(a);
   return p.nsplit <= 1 ? 0 : (int64_t)p.nsplit * a.batch * a.heads * a.q_len * (a.head_dim + 2) * 4;
 }
@@ -1157,20 +1412,48 @@ static void attention_bf16(const crnn_cross_attention_args& a, const AttnPlan& p
   else if (p.kw == 4) attention_bf16<DP, 1, 4>(a, p.nsplit, s);
   else attention_bf16<DP, 1, 1>(a, p.nsplit, s);
 }
+template <int TYPE, int LPK, int R>
+static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
+  constexpr int U = R == 4 || LPK == 4 ? 4 : 8;   // loads of each in a chunk: registers for two chunks and four rows are short
+  const int64_t total = a.batch * a.kv_heads * p.nsplit;
+  const dim3 g((unsigned)((total + 7) / 8 * 8));
+  if (p.kw == 1) hipLaunchKernelGGL((attention_few_kernel<TYPE, LPK, U, R, 1>), g, dim3(64), 0, s, a, p.nsplit);
+  else hipLaunchKernelGGL((attention_few_kernel<TYPE, LPK, U, R, 4>), g, dim3(256), 0, s, a, p.nsplit);
+}
+template <int TYPE, int LPK>
+static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
+  const int64_t rows = a.q_len * (a.heads / a.kv_heads);
+  if (rows == 1) attention_few<TYPE, LPK, 1>(a, p, s);
+  else if (rows == 2) attention_few<TYPE, LPK, 2>(a, p, s);
+  else attention_few<TYPE, LPK, 4>(a, p, s);
+}
+template <int TYPE>
+static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
+  const int chunks = a.head_dim / (TYPE == CRNN_BF16 ? 8 : 4);
+  if (chunks <= 4) attention_few<TYPE, 4>(a, p, s);
+  else if (chunks <= 8) attention_few<TYPE, 8>(a, p, s);
+  else if (chunks <= 16) attention_few<TYPE, 16>(a, p, s);
+  else if constexpr (TYPE == CRNN_FP32) attention_few<TYPE, 32>(a, p, s);
+}
+
+template <int TYPE, int LP>
+static void attention_join(const crnn_cross_attention_args& a, int nsplit, dim3 g, hipStream_t s) {
+  hipLaunchKernelGGL((attention_join_kernel<TYPE, LP>), g, dim3(256), 0, s, a, nsplit);
+}
 
 void launch_cross_attention(const crnn_cross_attention_args& a, hipStream_t s) {
   const int64_t rows = a.q_len * (a.heads / a.kv_heads);
   const int64_t blocks = a.batch * a.kv_heads * ((rows + 31) / 32);
-  if (attention_chunks(a) && attention_aligned(a) && (blocks < (1 << 22) || a.batch > 1)) {
+  if (!attention_any(a) && attention_aligned(a) && (blocks < (1 << 22) || a.batch > 1)) {
     if (blocks >= 1 << 22) {   // a launch has fewer than 2^32 threads: half the batch at a time (so many blocks use no workspace)
+      const int64_t e = a.type == CRNN_BF16 ? 2 : 4, n = a.batch / 2;
       crnn_cross_attention_args h[2] = {a, a};
-      const int64_t n = a.batch / 2;
       h[0].batch = n;
       h[1].batch = a.batch - n;
-      h[1].q = (const __bf16*)a.q + n * a.q_stride[0];
-      h[1].k = (const __bf16*)a.k + n * a.k_stride[0];
-      h[1].v = (const __bf16*)a.v + n * a.v_stride[0];
-      h[1].out = (__bf16*)a.out + n * a.out_stride[0];
+      h[1].q = (const char*)a.q + n * a.q_stride[0] * e;
+      h[1].k = (const char*)a.k + n * a.k_stride[0] * e;
+      h[1].v = (const char*)a.v + n * a.v_stride[0] * e;
+      h[1].out = (char*)a.out + n * a.out_stride[0] * e;
       if (a.lengths) h[1].lengths = a.lengths + n;
       if (a.mask) h[1].mask = a.mask + n * a.mask_stride;
       launch_cross_attention(h[0], s);
@@ -1178,11 +1461,16 @@ void launch_cross_attention(const crnn_cross_attention_args& a, hipStream_t s) {
       return;
     }
     const AttnPlan p = attention_plan(a);
-    if (a.head_dim <= 32) attention_bf16<32>(a, p, s);
+    if (p.rw == 0) a.type == CRNN_BF16 ? attention_few<CRNN_BF16>(a, p, s) : attention_few<CRNN_FP32>(a, p, s);
+    else if (a.head_dim <= 32) attention_bf16<32>(a, p, s);
     else if (a.head_dim <= 64) attention_bf16<64>(a, p, s);
     else if (a.head_dim <= 96) attention_bf16<96>(a, p, s);
     else attention_bf16<128>(a, p, s);
-    if (p.nsplit > 1) hipLaunchKernelGGL((attention_join_kernel<CRNN_BF16>), grid_for((a.batch * a.heads * a.q_len * a.head_dim + 255) / 256), dim3(256), 0, s, a, p.nsplit);
+    if (p.nsplit > 1) {
+      const dim3 g = grid_for(a.batch * a.heads * a.q_len);
+      if (a.type == CRNN_BF16) a.head_dim <= 64 ? attention_join<CRNN_BF16, 16>(a, p.nsplit, g, s) : attention_join<CRNN_BF16, 32>(a, p.nsplit, g, s);
+      else a.head_dim <= 64 ? attention_join<CRNN_FP32, 16>(a, p.nsplit, g, s) : attention_join<CRNN_FP32, 32>(a, p.nsplit, g, s);
+    }
     return;
   }
   const dim3 g = grid_for(a.batch * a.kv_heads * ((rows + 15) / 16)), b(256);

@@ -124,12 +124,24 @@ def test_line_attention_checks_its_weights():
         LineAttention(None, w, heads=4, kv_heads=3)
 
 
+def test_packed_arguments_are_the_structs():
+    from ocr_amd.crnn import seq_ops
+    for packer, struct in ((seq_ops._LINEAR, _capi.LinearArgs), (seq_ops._RMS_NORM, _capi.RmsNormArgs), (seq_ops._CROSS_ATTENTION, _capi.CrossAttentionArgs)):
+        assert packer.size == C.sizeof(struct)
+        values, flat = [], []
+        for i, (name, kind) in enumerate(struct._fields_):
+            v = i + 1.5 if kind is C.c_float else kind(i + 1, i + 51, i + 101) if kind is _capi.I64x3 else i + 1
+            values.append(v)
+            flat += list(v) if kind is _capi.I64x3 else [v]
+        assert packer.pack(*flat) == bytes(struct(*values))
+
+
 def test_rows_of_a_tensor():
     from ocr_amd.crnn.seq_ops import SequenceOps
     rows = SequenceOps._rows
     t = torch.zeros(6, 5, 32)
     assert rows("f", "t", t, 32) == (30, 32) and rows("f", "t", t[:, 0], 32) == (6, 160) and rows("f", "t", t[:, :, :16], 16) == (30, 32)
-    assert rows("f", "t", t[0, 0], 32) == (1, 32) and rows("f", "t", t[:, :0], 32)[0] == 0 and rows("f", "t", t[:1, 2:3], 32) == (1, 32)
+    assert rows("f", "t", t[0, 0], 32) == (1, 32) and rows("f", "t", t[:1, 0], 32) == (1, 32) and rows("f", "t", t[:, :0], 32)[0] == 0 and rows("f", "t", t[:1, 2:3], 32) == (1, 32)
     assert rows("f", "t", t[0, :1].expand(7, 32), 32) == (7, 0)
     with pytest.raises(ValueError):
         rows("f", "t", t[:, :4], 32)
