@@ -870,22 +870,26 @@ struct SplitRow {
   }
 };
 
-// bf16, head_dim and strides in whole 16-byte chunks.  Four waves (or one): RW of them side by side over 32 rows each, KW of
-// them over different tiles of KT keys; head_dim padded to DP.  Both products run transposed, S^T = K Q^T and O^T = V^T P^T
+// head_dim and strides in whole 16-byte chunks.  RW waves side by side over 32 rows each, KW times as many over different tiles
+// of KT keys; head_dim padded to DP.  Both products run transposed, S^T = K Q^T and O^T = V^T P^T
 // (v_mfma_f32_32x32x16_bf16): a lane then holds one query row in both results, so maximum, sum and rescaling are per lane, and
 // the exponentials are the second product's operand as they stand, because its sum may run over the keys in any order: register
 // r of S^T is key (r & 3) + 8 (r >> 2) + 4 (lane >> 5), and ds_read_tr16_b64 takes V's columns for four such keys at a time.
 // K and V tiles go straight to LDS, two stages; 16-byte chunk c of row j sits at chunk c ^ swizzle(j), which spreads what is
-// read at once -- 16 rows of K, 64 bytes of four rows of V -- over the 256 bytes that LDS serves in a cycle.  Keys that are left out are never loaded: their
+// read at once -- 16 rows of K, 64 bytes of four rows of V -- over the 256 bytes that LDS serves in a cycle.  fp32 runs the same
+// way on v_mfma_f32_32x32x2_f32: a 16-byte chunk feeds four of them, register r of S^T is one's second operand, and V is read
+// value by value (its rows r and r + 4 half a row apart).  Keys that are left out are never loaded: their
 // offset lies outside the resource, LDS gets zeros, and their score is -inf.
 // With nsplit > 1 workgroups share the keys of one row block and leave (O, M, L) for attention_join_kernel.
-template <int DP, int RW, int KW, int KT>
-__global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const crnn_cross_attention_args a, int nsplit) {
-  constexpr int NCH = DP / 8, ROWB = DP * 2, TILE = KT * ROWB, NW = RW * KW;   // chunks of a row, bytes of a row and of a tile
+template <int TYPE, int DP, int RW, int KW, int KT>
+__global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const crnn_cross_attention_args a, int nsplit) {
+  typedef typename TypeOf<TYPE>::t T;
+  constexpr int ES = sizeof(T), EPC = 16 / ES, ROWB = DP * ES, NCH = ROWB / 16, TILE = KT * ROWB;   // values of a chunk, bytes and chunks of a row
   constexpr int LOADS = TILE / 1024;                                          // dma16 instructions a tile, shared by RW waves
   __shared__ __attribute__((aligned(1024))) unsigned char smem[KW * 4 * TILE];   // [KW][2 stages][K, V]
   static_assert(KW == 1 || sizeof(smem) >= (RW * DP * 32 + RW * 64) * 4, "the join's exchange fits the tiles");
-  if constexpr (sizeof(smem) > 80 * 1024) CRNN_WHOLE_REGISTER_FILE();   // (one workgroup a CU: the compiler uses AccVGPRs)
+  // (LDS leaves a SIMD one wave: the compiler then uses AccVGPRs)
+  if constexpr (sizeof(smem) > 80 * 1024 || (ES == 4 && 163840 / sizeof(smem) * RW * KW < 8)) CRNN_WHOLE_REGISTER_FILE();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int kw = wave / RW, rw = wave % RW;
   const int G = a.heads / a.kv_heads, D = a.head_dim;
@@ -899,30 +903,32 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const c
   // this workgroup's keys: whole steps of KW tiles
   const int steps_all = (len + KT * KW - 1) / (KT * KW), steps_per = (steps_all + nsplit - 1) / nsplit;
   const int step0 = min(sp * steps_per, steps_all), steps = min(steps_per, steps_all - step0);
-  const __bf16* kp = (const __bf16*)a.k + b * a.k_stride[0] + g * a.k_stride[2];
-  const __bf16* vp = (const __bf16*)a.v + b * a.v_stride[0] + g * a.v_stride[2];
+  const T* kp = (const T*)a.k + b * a.k_stride[0] + g * a.k_stride[2];
+  const T* vp = (const T*)a.v + b * a.v_stride[0] + g * a.v_stride[2];
   const uint8_t* mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
 
-  // query rows, as the second operand: lane & 31 the row, 8 values from 16 kk + 8 half.  A negative scale turns their sign
+  // query rows, as the second operand: lane & 31 the row, its chunks 2 kk + half.  A negative scale turns their sign
   const float sc = fmaxf(fabsf(a.scale), 1e-38f) * 1.4426950408889634f;
   const int64_t row = rb * 32 * RW + rw * 32 + (lane & 31);
   const bool live = row < rows;
-  bf16x8 q[DP / 16];
+  i32x4 q[NCH / 2];
   {
-    const __bf16* qp = (const __bf16*)a.q + b * a.q_stride[0] + (live ? row / G : 0) * a.q_stride[1] + (g * G + (live ? row % G : 0)) * a.q_stride[2];
-    const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
+    const T* qp = (const T*)a.q + b * a.q_stride[0] + (live ? row / G : 0) * a.q_stride[1] + (g * G + (live ? row % G : 0)) * a.q_stride[2];
+    const unsigned flip = a.scale < 0.f ? (ES == 2 ? 0x80008000u : 0x80000000u) : 0u;
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; kk++) {
-      const int d = 16 * kk + 8 * half;
-      i32x4 u = {0, 0, 0, 0};
-      if (live && d < D) u = *(const i32x4*)(qp + d);
+    for (int kk = 0; kk < NCH / 2; kk++) {
+      const int d = (2 * kk + half) * EPC;
+      q[kk] = i32x4{0, 0, 0, 0};
+      if (live && d < D) q[kk] = *(const i32x4*)(qp + d);
 #pragma unroll
-      for (int i = 0; i < 4; i++) u[i] ^= flip;
-      q[kk] = __builtin_bit_cast(bf16x8, u);
+      for (int i = 0; i < 4; i++) q[kk][i] ^= flip;
     }
   }
-  auto swz_k = [](int r) { return NCH == 16 ? r & 15 : NCH == 8 ? (r >> 1) & 7 : (r >> 2) & 3; };
-  auto swz_v = [](int r) { return NCH == 16 ? 4 * (r & 3) : NCH == 8 ? 2 * (r & 2) : 0; };
+  auto swz_k = [](int r) { return NCH % 16 == 0 ? r & 15 : NCH % 8 == 0 ? (r >> 1) & 7 : (r >> 2) & 3; };
+  auto swz_v = [](int r) {
+    if (ES == 4) return NCH % 16 == 0 ? 2 * (r & 4) : 0;
+    return NCH == 16 ? 4 * (r & 3) : NCH == 8 ? 2 * (r & 2) : 0;
+  };
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem + kw * 4 * TILE;
   const unsigned char* base = smem + kw * 4 * TILE;
 
@@ -949,8 +955,8 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const c
       const int pos = n * 64 + lane, r = pos / NCH, c = pos % NCH;
       const bool key = (w >> r) & 1;
       const int ck = c ^ swz_k(r), cv = c ^ swz_v(r);
-      dma16(rk, lds0 + stage * 2 * TILE + n * 1024, key && ck * 8 < D ? (unsigned)(r * (int)a.k_stride[1] + ck * 8) * 2u : OUTSIDE);
-      dma16(rv, lds0 + stage * 2 * TILE + TILE + n * 1024, key && cv * 8 < D ? (unsigned)(r * (int)a.v_stride[1] + cv * 8) * 2u : OUTSIDE);
+      dma16(rk, lds0 + stage * 2 * TILE + n * 1024, key && ck * EPC < D ? (unsigned)(r * (int)a.k_stride[1] + ck * EPC) * ES : OUTSIDE);
+      dma16(rv, lds0 + stage * 2 * TILE + TILE + n * 1024, key && cv * EPC < D ? (unsigned)(r * (int)a.v_stride[1] + cv * EPC) * ES : OUTSIDE);
     }
   };
 
@@ -985,9 +991,9 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const c
         for (int r = 0; r < 16; r++) s[kb][r] = 0.f;
         const int r = kb * 32 + (lane & 31);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; kk++) {
-          const bf16x8 f = *(const bf16x8*)(kt + r * ROWB + (((2 * kk + half) ^ swz_k(r)) << 4));
-          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, q[kk], s[kb], 0, 0, 0);
+        for (int kk = 0; kk < NCH / 2; kk++) {
+          const i32x4 f = *(const i32x4*)(kt + r * ROWB + (((2 * kk + half) ^ swz_k(r)) << 4));
+          s[kb] = Slice<TYPE>::mfma(__builtin_bit_cast(typename Slice<TYPE>::frag, f), __builtin_bit_cast(typename Slice<TYPE>::frag, q[kk]), s[kb]);
         }
       }
       const unsigned long long full = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
@@ -1022,21 +1028,33 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const c
           s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], sc, -Ms));
           L += s[kb][r];
         }
+        if constexpr (TYPE == CRNN_BF16) {
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          bf16x8 pj;
+          for (int j = 0; j < 2; j++) {
+            bf16x8 pj;
 #pragma unroll
-          for (int i = 0; i < 8; i++) pj[i] = (__bf16)s[kb][8 * j + i];
+            for (int i = 0; i < 8; i++) pj[i] = (__bf16)s[kb][8 * j + i];
 #pragma unroll
-          for (int db = 0; db < DP / 32; db++) {
-            s16x4 f[2];
+            for (int db = 0; db < DP / 32; db++) {
+              s16x4 f[2];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-              const int r = kb * 32 + 16 * j + 8 * i + 4 * half + ((lane & 15) >> 2), c = db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-              f[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + r * ROWB + ((c ^ swz_v(r)) << 4) + (lane & 1) * 8));
+              for (int i = 0; i < 2; i++) {
+                const int r = kb * 32 + 16 * j + 8 * i + 4 * half + ((lane & 15) >> 2), c = db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                f[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + r * ROWB + ((c ^ swz_v(r)) << 4) + (lane & 1) * 8));
+              }
+              const s16x8 v8 = __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7);
+              o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v8), pj, o[db], 0, 0, 0);
             }
-            const s16x8 v8 = __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7);
-            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v8), pj, o[db], 0, 0, 0);
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int j = kb * 32 + acc_row(r, lane);
+#pragma unroll
+            for (int db = 0; db < DP / 32; db++) {
+              const int d = db * 32 + (lane & 31);
+              o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(*(const float*)(vt + j * ROWB + (((d >> 2) ^ swz_v(j)) << 4) + (d & 3) * 4), s[kb][r], o[db], 0, 0, 0);
+            }
           }
         }
       }
@@ -1081,20 +1099,21 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_bf16_kernel(const c
     for (int i = 0; i < DP / 32; i++)
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
-        const int d = i * 32 + acc_row(r, lane);   // four neighbours; head_dim is a multiple of 8
+        const int d = i * 32 + acc_row(r, lane);   // four neighbours; head_dim is a multiple of 4
         if (d < D) *(f32x4*)(w.o + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
       }
     if (half == 0) w.ml[0] = Me, w.ml[1] = L;
     return;
   }
-  __bf16* out = (__bf16*)a.out + b * a.out_stride[0] + row / G * a.out_stride[1] + (g * G + row % G) * a.out_stride[2];
+  T* out = (T*)a.out + b * a.out_stride[0] + row / G * a.out_stride[1] + (g * G + row % G) * a.out_stride[2];
   const float il = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
   for (int i = 0; i < DP / 32; i++)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-      const int d = i * 32 + acc_row(r, lane);   // four neighbours; head_dim is a multiple of 8
-      if (d < D) *(bf16x4u*)(out + d) = bf16x4u{(__bf16)(o[i][r] * il), (__bf16)(o[i][r + 1] * il), (__bf16)(o[i][r + 2] * il), (__bf16)(o[i][r + 3] * il)};
+      typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+      const int d = i * 32 + acc_row(r, lane);   // four neighbours; head_dim is a multiple of 4
+      if (d < D) *(T4*)(out + d) = T4{(T)(o[i][r] * il), (T)(o[i][r + 1] * il), (T)(o[i][r + 2] * il), (T)(o[i][r + 3] * il)};
     }
 }
 
@@ -1375,8 +1394,8 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
     keys = 64 * p.kw;
   } else {
     p.rw = rows > 64 ? 4 : rows > 32 ? 2 : 1;
-    p.kw = 4 / p.rw;
-    const int kt = p.rw == 4 ? 64 : 32;
+    p.kw = a.type == CRNN_BF16 ? 4 / p.rw : p.rw == 1 ? 2 : 1;
+    const int kt = a.type == CRNN_BF16 && p.rw == 4 ? 64 : 32;
     if (p.rw == 1 && a.kv_len <= 4 * kt && bg >= 1024) p.kw = 1;
     blocks = bg * ((rows + 32 * p.rw - 1) / (32 * p.rw));
     keys = kt * p.kw;
@@ -1388,29 +1407,32 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
   p.nsplit = (int)(ns < 1 ? 1 : ns > MAX_SPLIT ? MAX_SPLIT : ns);
   return p;
 }
-static bool attention_any(const crnn_cross_attention_args& a) {   // shapes that only attention_any_kernel takes
-  if (!attention_chunks(a)) return true;
-  return a.type == CRNN_FP32 && a.q_len * (a.heads / a.kv_heads) > 4;
-}
-
 int64_t cross_attention_workspace(const crnn_cross_attention_args& a) {
-  if (attention_any(a)) return 0;
+  if (!attention_chunks(a)) return 0;
   const AttnPlan p = attention_plan(a);
   return p.nsplit <= 1 ? 0 : (int64_t)p.nsplit * a.batch * a.heads * a.q_len * (a.head_dim + 2) * 4;
 }
 
-template <int DP, int RW, int KW>
-static void attention_bf16(const crnn_cross_attention_args& a, int nsplit, hipStream_t s) {
-  constexpr int KT = RW == 4 ? 64 : 32;
+template <int TYPE, int DP, int RW, int KW>
+static void attention_tile(const crnn_cross_attention_args& a, int nsplit, hipStream_t s) {
+  constexpr int KT = TYPE == CRNN_BF16 && RW == 4 ? 64 : 32;
   const int64_t rows = a.q_len * (a.heads / a.kv_heads), total = a.batch * a.kv_heads * ((rows + 32 * RW - 1) / (32 * RW)) * nsplit;
-  hipLaunchKernelGGL((attention_bf16_kernel<DP, RW, KW, KT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * RW * KW), 0, s, a, nsplit);
+  hipLaunchKernelGGL((attention_tile_kernel<TYPE, DP, RW, KW, KT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * RW * KW), 0, s, a, nsplit);
 }
-template <int DP>
-static void attention_bf16(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
-  if (p.rw == 4) attention_bf16<DP, 4, 1>(a, p.nsplit, s);
-  else if (p.rw == 2) attention_bf16<DP, 2, 2>(a, p.nsplit, s);
-  else if (p.kw == 4) attention_bf16<DP, 1, 4>(a, p.nsplit, s);
-  else attention_bf16<DP, 1, 1>(a, p.nsplit, s);
+template <int TYPE, int DP>
+static void attention_tile(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
+  constexpr int K = TYPE == CRNN_BF16 ? 2 : 1;   // (fp32 tiles take twice the LDS)
+  if (p.rw == 4) attention_tile<TYPE, DP, 4, 1>(a, p.nsplit, s);
+  else if (p.rw == 2) attention_tile<TYPE, DP, 2, K>(a, p.nsplit, s);
+  else if (p.kw > 1) attention_tile<TYPE, DP, 1, 2 * K>(a, p.nsplit, s);
+  else attention_tile<TYPE, DP, 1, 1>(a, p.nsplit, s);
+}
+template <int TYPE>
+static void attention_tile(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
+  if (a.head_dim <= 32) attention_tile<TYPE, 32>(a, p, s);
+  else if (a.head_dim <= 64) attention_tile<TYPE, 64>(a, p, s);
+  else if (a.head_dim <= 96) attention_tile<TYPE, 96>(a, p, s);
+  else attention_tile<TYPE, 128>(a, p, s);
 }
 template <int TYPE, int LPK, int R>
 static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
@@ -1444,7 +1466,7 @@ static void attention_join(const crnn_cross_attention_args& a, int nsplit, dim3 
 void launch_cross_attention(const crnn_cross_attention_args& a, hipStream_t s) {
   const int64_t rows = a.q_len * (a.heads / a.kv_heads);
   const int64_t blocks = a.batch * a.kv_heads * ((rows + 31) / 32);
-  if (!attention_any(a) && attention_aligned(a) && (blocks < (1 << 22) || a.batch > 1)) {
+  if (attention_chunks(a) && attention_aligned(a) && (blocks < (1 << 22) || a.batch > 1)) {
     if (blocks >= 1 << 22) {   // a launch has fewer than 2^32 threads: half the batch at a time (so many blocks use no workspace)
       const int64_t e = a.type == CRNN_BF16 ? 2 : 4, n = a.batch / 2;
       crnn_cross_attention_args h[2] = {a, a};
@@ -1462,10 +1484,7 @@ void launch_cross_attention(const crnn_cross_attention_args& a, hipStream_t s) {
     }
     const AttnPlan p = attention_plan(a);
     if (p.rw == 0) a.type == CRNN_BF16 ? attention_few<CRNN_BF16>(a, p, s) : attention_few<CRNN_FP32>(a, p, s);
-    else if (a.head_dim <= 32) attention_bf16<32>(a, p, s);
-    else if (a.head_dim <= 64) attention_bf16<64>(a, p, s);
-    else if (a.head_dim <= 96) attention_bf16<96>(a, p, s);
-    else attention_bf16<128>(a, p, s);
+    else a.type == CRNN_BF16 ? attention_tile<CRNN_BF16>(a, p, s) : attention_tile<CRNN_FP32>(a, p, s);
     if (p.nsplit > 1) {
       const dim3 g = grid_for(a.batch * a.heads * a.q_len);
       if (a.type == CRNN_BF16) a.head_dim <= 64 ? attention_join<CRNN_BF16, 16>(a, p.nsplit, g, s) : attention_join<CRNN_BF16, 32>(a, p.nsplit, g, s);
