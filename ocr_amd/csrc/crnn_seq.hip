@@ -31,6 +31,12 @@ template <> struct TypeOf<CRNN_E4M3> { typedef e4m3 t; };
 // FIRST operand's index
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
 
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
 // erf by Abramowitz & Stegun 7.1.26: 1 - (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p |x|), off by at most 1.5e-7 -- what
 // 1 + erf loses to rounding is of that size.  (erff and expf with a division: 94 instead of 62 + 8 us for 18176 x 512 x 2048.)
 __device__ __forceinline__ float gelu(float v) {
@@ -233,17 +239,20 @@ template <int N> __device__ __forceinline__ void wait_loads() {   // all but the
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
-template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST>
-__global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a, int wide) {
+template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST, int KG>
+__global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a, int wide) {
   typedef Slice<IN> S;
   typedef typename TypeOf<OUT>::t TO;
   constexpr int ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1, NKS = RB / S::KB, RPL = 1024 / RB;   // slices of a step, rows of a load
   constexpr int NW = 2 * WN, BM = 64 * MT, BN = 32 * WN * NT, STAGE = (BM + BN) * RB;
   constexpr int LX = BM / (RPL * NW), LT = (BM + BN) / (RPL * NW);   // dma16 instructions of a wave and step: of x, all
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[NST * STAGE];
-  static_assert(sizeof(smem) >= NW * 32 * (32 * NT * 4 + 16), "the epilogue's exchange fits");
+  constexpr int JOIN = (KG - 1) * NW * MT * NT * 4096;   // bytes of the other groups' sums
+  __shared__ __attribute__((aligned(1024))) unsigned char smem_all[KG * NST * STAGE];
+  static_assert(sizeof(smem_all) >= JOIN + NW * 32 * (32 * NT * 4 + 16), "the epilogue's exchange fits");
   if constexpr (MT * NT > 8) CRNN_WHOLE_REGISTER_FILE();
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, half = lane >> 5;
+  const int kg = __builtin_amdgcn_readfirstlane(tid >> 6) / NW;
+  unsigned char* smem = smem_all + kg * NST * STAGE;
   const int wm = wave / WN, wn = wave % WN;
   // Tiles in groups of eight rows of tiles, column by column; a run of consecutive tiles per XCD, so that the 32 tiles it works
   // on at a time are 8 x 4 and share their operands in its L2
@@ -254,7 +263,7 @@ __global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_ker
   const int64_t m0 = (int64_t)(grp * 8 + in % gm) * BM, n0 = (int64_t)(in / gm) * BN;
 
   const unsigned kbytes = (unsigned)a.k * ES;
-  const int nk = (int)((kbytes + RB - 1) / RB);
+  const int nk = (int)((kbytes + RB * KG - 1) / (RB * KG));   // steps of a group: KG t + kg
   const i32x4 rx = resource((const char*)a.x + m0 * a.ldx * ES), rw = resource((const char*)a.w + n0 * a.ldw * ES);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
   // lane l of load i of this wave: row r = (wave + NW i) RPL + l / (RB / 16), chunk (l mod RB / 16) ^ swizzle(r), the same for all i
@@ -271,7 +280,7 @@ __global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_ker
   }
   // load i of LT of `step` into `stage` (x before w); past the end of a row, zeros
   auto load = [&](int step, int stage, int i) __attribute__((always_inline)) {
-    const unsigned kb = (unsigned)step * RB, to = lds0 + stage * STAGE + (i < LX ? (wave + NW * i) * 1024 : BM * RB + (wave + NW * (i - LX)) * 1024);
+    const unsigned kb = (unsigned)(step * KG + kg) * RB, to = lds0 + stage * STAGE + (i < LX ? (wave + NW * i) * 1024 : BM * RB + (wave + NW * (i - LX)) * 1024);
     dma16(i < LX ? rx : rw, to, kb + cb < kbytes ? off[i] : OUTSIDE, kb);
   };
   f32x16 acc[NT][MT];
@@ -339,9 +348,30 @@ __global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_ker
   // Epilogue: the sums of 32 rows at a time go through LDS (each wave has its own part), after which a lane holds eight
   // neighbours of a row: bias, activation and residual happen there, and rows leave as whole lines.
   __syncthreads();   // (nobody reads the stages any more)
+  if constexpr (KG > 1) {   // the groups' sums, added in their order
+    float* part = (float*)smem_all + (wave * MT * NT * 16) * 64 + lane;
+    if (kg > 0) {
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) part[((kg - 1) * NW * MT * NT * 16 + (i * MT + j) * 16 + r) * 64] = acc[i][j][r];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int k = 0; k < KG - 1; k++)
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[i][j][r] += part[(k * NW * MT * NT * 16 + (i * MT + j) * 16 + r) * 64];
+  }
   constexpr int PITCH = 32 * NT * 4 + 16;
   constexpr int LPR = 4 * NT, RPI = 64 / LPR, RI = 32 / RPI;   // lanes a row, rows at a time, times
-  unsigned char* ex = smem + wave * 32 * PITCH;
+  unsigned char* ex = smem_all + JOIN + wave * 32 * PITCH;
   const int c = (lane % LPR) * 8;
   const int64_t n = n0 + wn * 32 * NT + c, left = a.n - n;
   const int64_t mw = m0 + wm * 32 * MT + lane / LPR;   // this lane's rows: mw + 32 j + RPI i
@@ -411,18 +441,18 @@ __global__ __launch_bounds__(128 * WN, MT * NT > 8 ? 1 : 2) void linear_tile_ker
 }
 
 // ---------------------------------------------------------------------------
-// linear, few rows (at most 64) of whole 16-byte chunks: 32 columns of y per workgroup, whose KW waves take 128 bytes of k of
+// linear, few rows (at most 32; called for 16) of whole 16-byte chunks: 32 columns of y per workgroup, whose KW waves take 128 bytes of k of
 // every row of w in turn and add up through LDS in a fixed order.  Bound by reading w, or by the way of the first bytes: no
 // LDS on the way in, every lane loads its operands as they lie (the products may be added in any order, so a lane's half of a
 // block is 64 neighbouring bytes), the next block's while this one is multiplied.  x is the first operand: lanes hold
 // neighbouring columns.
 // ---------------------------------------------------------------------------
-template <int IN, int OUT, int MT, int KW>
+template <int IN, int OUT, int KW>
 __global__ __launch_bounds__(64 * KW, 2) void linear_rows_kernel(const crnn_linear_args a) {
   typedef typename TypeOf<OUT>::t TO;
   typedef Slice<IN> S;
   constexpr int ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1;
-  __shared__ float part[KW][MT * 16][64];
+  __shared__ float part[KW][16][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int64_t n0 = (int64_t)blockIdx.x * 32;
   const unsigned kbytes = (unsigned)a.k * ES;
@@ -430,37 +460,30 @@ __global__ __launch_bounds__(64 * KW, 2) void linear_rows_kernel(const crnn_line
   const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)a.x, 0, 0x7FFFFFFF, 0x00020000);
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.w + n0 * a.ldw * ES), 0, 0x7FFFFFFF, 0x00020000);
   const unsigned ow = n0 + (lane & 31) < a.n ? (unsigned)((lane & 31) * (int)a.ldw * ES) + half * 64u : OUTSIDE;
-  unsigned ox[MT];
+  const unsigned ox = (lane & 31) < a.m ? (unsigned)((lane & 31) * (int)a.ldx * ES) + half * 64u : OUTSIDE;
+  f32x16 acc;
 #pragma unroll
-  for (int j = 0; j < MT; j++) ox[j] = 32 * j + (lane & 31) < a.m ? (unsigned)((32 * j + (lane & 31)) * (int)a.ldx * ES) + half * 64u : OUTSIDE;
-  f32x16 acc[MT];
-#pragma unroll
-  for (int j = 0; j < MT; j++)
-#pragma unroll
-    for (int r = 0; r < 16; r++) acc[j][r] = 0.f;
-  i32x4 w[2][4], x[2][MT][4];
+  for (int r = 0; r < 16; r++) acc[r] = 0.f;
+  i32x4 w[2][4], x[2][4];
   auto load = [&](int set, int blk) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       const unsigned kb = (unsigned)blk * 128 + c * 16;
       const bool in = kb + half * 64u < kbytes;   // (a block past the end: zeros)
       w[set][c] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? ow + kb : OUTSIDE, 0, 0);
-#pragma unroll
-      for (int j = 0; j < MT; j++) x[set][j][c] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? ox[j] + kb : OUTSIDE, 0, 0);
+      x[set][c] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? ox + kb : OUTSIDE, 0, 0);
     }
   };
   auto multiply = [&](int set) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < MT; j++)
-#pragma unroll
-      for (int c = 0; c < 4; c += IN == CRNN_E4M3 ? 2 : 1) {
-        if constexpr (IN == CRNN_E4M3) {
-          const i32x4 x0 = x[set][j][c], x1 = x[set][j][c + 1], w0 = w[set][c], w1 = w[set][c + 1];
-          acc[j] = S::mfma(i32x8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]}, i32x8{w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]}, acc[j]);
-        } else {
-          acc[j] = S::mfma(__builtin_bit_cast(typename S::frag, x[set][j][c]), __builtin_bit_cast(typename S::frag, w[set][c]), acc[j]);
-        }
+    for (int c = 0; c < 4; c += IN == CRNN_E4M3 ? 2 : 1) {
+      if constexpr (IN == CRNN_E4M3) {
+        const i32x4 x0 = x[set][c], x1 = x[set][c + 1], w0 = w[set][c], w1 = w[set][c + 1];
+        acc = S::mfma(i32x8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]}, i32x8{w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]}, acc);
+      } else {
+        acc = S::mfma(__builtin_bit_cast(typename S::frag, x[set][c]), __builtin_bit_cast(typename S::frag, w[set][c]), acc);
       }
+    }
   };
   load(0, wave);
   for (int blk = wave; blk < nb; blk += 2 * KW) {
@@ -470,15 +493,13 @@ __global__ __launch_bounds__(64 * KW, 2) void linear_rows_kernel(const crnn_line
     multiply(1);
   }
 #pragma unroll
-  for (int j = 0; j < MT; j++)
-#pragma unroll
-    for (int r = 0; r < 16; r++) part[wave][j * 16 + r][lane] = acc[j][r];
+  for (int r = 0; r < 16; r++) part[wave][r][lane] = acc[r];
   __syncthreads();
   const int64_t n = n0 + (lane & 31);
   if (n >= a.n) return;
   const float bias = a.bias ? a.bias[n] : 0.f, wsc = IN == CRNN_E4M3 && a.w_scale ? a.w_scale[n] : 1.f;
-  for (int i = wave; i < MT * 16; i += KW) {
-    const int m = (i >> 4) * 32 + acc_row(i & 15, lane);
+  for (int i = wave; i < 16; i += KW) {
+    const int m = acc_row(i, lane);
     if (m >= a.m) continue;
     float v = 0.f;
 #pragma unroll
@@ -490,6 +511,78 @@ __global__ __launch_bounds__(64 * KW, 2) void linear_rows_kernel(const crnn_line
   }
 }
 
+// One to four rows: a wave per NC columns of y, its lanes side by side along k, 16 bytes of every column and row each; fp32 FMAs.
+// Nothing but the first bytes' way and the reading of w: four loads of each column are on their way at a time.
+template <int IN, int OUT, int M, int NC>
+__global__ __launch_bounds__(256, 2) void linear_vector_kernel(const crnn_linear_args a) {
+  typedef typename TypeOf<IN>::t T;
+  typedef typename TypeOf<OUT>::t TO;
+  constexpr int ES = sizeof(T), EPC = 16 / ES, U = 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * NC;
+  if (n0 >= a.n) return;
+  const unsigned kbytes = (unsigned)a.k * ES;
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)a.x, 0, 0x7FFFFFFF, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.w + n0 * a.ldw * ES), 0, 0x7FFFFFFF, 0x00020000);
+  auto widen = [](i32x4 u, float (&v)[EPC]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (ES == 4) v[i] = __uint_as_float((unsigned)u[i]);
+      else if constexpr (ES == 2) v[2 * i] = __uint_as_float((unsigned)u[i] << 16), v[2 * i + 1] = __uint_as_float((unsigned)u[i] & 0xFFFF0000u);
+      else v[4 * i] = __builtin_amdgcn_cvt_f32_fp8(u[i], 0), v[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(u[i], 1), v[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(u[i], 2), v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(u[i], 3);
+    }
+  };
+  float acc[M][NC];
+#pragma unroll
+  for (int m = 0; m < M; m++)
+#pragma unroll
+    for (int c = 0; c < NC; c++) acc[m][c] = 0.f;
+  for (unsigned k0 = lane * 16; k0 < kbytes; k0 += U * 1024) {
+    i32x4 w[U][NC], x[U][M];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const unsigned kb = k0 + u * 1024;
+      const bool in = kb < kbytes;
+#pragma unroll
+      for (int c = 0; c < NC; c++) w[u][c] = __builtin_amdgcn_raw_buffer_load_b128(rw, in && n0 + c < a.n ? (unsigned)(c * (int)a.ldw * ES) + kb : OUTSIDE, 0, 0);
+#pragma unroll
+      for (int m = 0; m < M; m++) x[u][m] = __builtin_amdgcn_raw_buffer_load_b128(rx, in && m < a.m ? (unsigned)(m * (int)a.ldx * ES) + kb : OUTSIDE, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float wv[NC][EPC], xv[M][EPC];
+#pragma unroll
+      for (int c = 0; c < NC; c++) widen(w[u][c], wv[c]);
+#pragma unroll
+      for (int m = 0; m < M; m++) widen(x[u][m], xv[m]);
+#pragma unroll
+      for (int m = 0; m < M; m++)
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+          for (int i = 0; i < EPC; i++) acc[m][c] = fmaf(xv[m][i], wv[c][i], acc[m][c]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < M; m++)
+#pragma unroll
+    for (int c = 0; c < NC; c++) acc[m][c] = wave_sum(acc[m][c]);
+  // lane m NC + c has the value of row m, column c
+  float v = 0.f;
+#pragma unroll
+  for (int m = 0; m < M; m++)
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+      if (lane == m * NC + c) v = acc[m][c];
+  const int m = lane / NC;
+  const int64_t n = n0 + lane % NC;
+  if (m >= M || m >= a.m || n >= a.n) return;
+  if (IN == CRNN_E4M3) v = v * (a.x_scale ? a.x_scale[m] : 1.f) * (a.w_scale ? a.w_scale[n] : 1.f);
+  v = activate(v + (a.bias ? a.bias[n] : 0.f), a.act);
+  if (a.residual) v += (float)((const TO*)a.residual)[m * a.ldr + n];
+  ((TO*)a.y)[m * a.ldy + n] = (TO)v;
+}
+
 // Rows of whole 16-byte chunks, and offsets within a tile below 2^31 bytes.
 static bool linear_chunks(const crnn_linear_args& a) {
   const int64_t es = a.in_type == CRNN_FP32 ? 4 : a.in_type == CRNN_BF16 ? 2 : 1, c = 16 / es;
@@ -498,13 +591,13 @@ static bool linear_chunks(const crnn_linear_args& a) {
          (256 * (a.ldx > a.ldw ? a.ldx : a.ldw) + a.k) * es < 0x7FFFF000;
 }
 
-template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST>
+template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST, int KG = 1>
 static void linear_tile(const crnn_linear_args& a, hipStream_t s) {
   const int64_t eo = OUT == CRNN_FP32 ? 4 : 2;
   auto chunks = [&](const void* p, int64_t ld) { return (((uintptr_t)p | (uintptr_t)(ld * eo)) & 15) == 0; };
   const int wide = chunks(a.y, a.ldy) && (!a.residual || chunks(a.residual, a.ldr));
   const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 32 * WN * NT - 1) / (32 * WN * NT));
-  hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT, WN, RB, NST>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(128 * WN), 0, s, a, wide);
+  hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT, WN, RB, NST, KG>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(128 * WN * KG), 0, s, a, wide);
 }
 template <int IN, int OUT>
 static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
@@ -513,32 +606,42 @@ static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
   // less use of what is loaded.  18176 x 512 x 2048: 256 rows 54 us, 192 rows 50, 128 x 128 59; 16384 x 4096 x 4096: 455, 488, 556.
   auto rounds = [&](int bm, int bn, int at_once) { return (double)(((a.m + bm - 1) / bm * ((a.n + bn - 1) / bn) + at_once - 1) / at_once); };
   const double c4 = 4.0 * rounds(256, 256, 256), c3 = 3.0 * rounds(192, 256, 256), c2 = 2.4 * rounds(128, 128, 512);
-  const int64_t small = ((a.m + 127) / 128) * ((a.n + 127) / 128);
+  const int64_t small = ((a.m + 127) / 128) * ((a.n + 127) / 128), tiny = ((a.m + 63) / 64) * ((a.n + 31) / 32);
   if constexpr (IN != CRNN_FP32) {
     if (c4 <= c3 && c4 <= c2) return linear_tile<IN, OUT, 4, 2, 4, 128, 2>(a, s), true;
     if (c3 <= c2) return linear_tile<IN, OUT, 3, 2, 4, 128, 2>(a, s), true;
   }
   if (small >= 256) linear_tile<IN, OUT, 2, 2, 2, 128, 2>(a, s);
-  else linear_tile<IN, OUT, 1, 1, 2, 128, 4>(a, s);
+  // (few small tiles: four groups of waves share k.  64 x 2048 x 2048 9.2 us, without 12.5; 300 x 512 x 5530 20 us, without 11)
+  else if (tiny <= 256) linear_tile<IN, OUT, 1, 1, 1, 128, 3, 4>(a, s);
+  else linear_tile<IN, OUT, 1, 1, 2, 128, 3>(a, s);
   return true;
 }
 
-template <int IN, int OUT, int MT>
+template <int IN, int OUT>
 static void linear_rows(const crnn_linear_args& a, hipStream_t s) {
   constexpr int ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1;
   const dim3 g((unsigned)((a.n + 31) / 32));
-  if (a.k * ES <= 1024) hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, MT, 4>), g, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, MT, 8>), g, dim3(512), 0, s, a);
+  if (a.k * ES <= 1024) hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, 4>), g, dim3(256), 0, s, a);
+  else if (a.k * ES <= 4096) hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, 8>), g, dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, 16>), g, dim3(1024), 0, s, a);
+}
+template <int IN, int OUT, int M>
+static void linear_vector(const crnn_linear_args& a, hipStream_t s) {
+  // (a wave for one column while that does not fill the chip four times over)
+  if (a.n <= 4096) hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 1>), dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 4>), dim3((unsigned)((a.n + 15) / 16)), dim3(256), 0, s, a);
 }
 
 template <int IN, int OUT>
 static void linear_of(const crnn_linear_args& a, hipStream_t s) {
   if constexpr (IN != CRNN_E4M3 || OUT == CRNN_BF16) {
     if (linear_chunks(a)) {
-      if (a.m <= 64 && a.n < 1 << 27) {
-        a.m <= 32 ? linear_rows<IN, OUT, 1>(a, s) : linear_rows<IN, OUT, 2>(a, s);
+      if (a.m <= 4 && a.n < 1 << 26) {
+        a.m == 1 ? linear_vector<IN, OUT, 1>(a, s) : a.m == 2 ? linear_vector<IN, OUT, 2>(a, s) : linear_vector<IN, OUT, 4>(a, s);
         return;
       }
+      if (a.m <= 16 && a.n < 1 << 27) return linear_rows<IN, OUT>(a, s);
       if (linear_tiles<IN, OUT>(a, s)) return;
     }
   }
@@ -556,11 +659,6 @@ void launch_linear(const crnn_linear_args& a, hipStream_t s) {
 // exact (rows around 1e-20 or above 1e18) it is taken again in 64 bits, and r is applied as a power of two near 1 / |t| and
 // the rest, so that no product on the way leaves the normal numbers.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
