@@ -224,6 +224,38 @@ template <> struct Slice<CRNN_FP32> {   // one 16-byte chunk a lane: four v_mfma
   }
 };
 
+// fp32 in three bfloat16 parts: x = h + m + l, each the leading 8 bits of what is left (cut, so the parts are exact and their
+// differences too).  Of the nine products the six largest are multiplied (v_mfma_f32_32x32x16_bf16 at 16 times the rate of the
+// f32 instructions); the others are below 2^-24 of the product.  An infinity makes h infinite and m NaN, and values near the
+// largest may overflow on the way: results that are not finite are computed again by linear_tile_kernel on the f32 instructions.
+struct Parts {
+  bf16x8 p[3];
+};
+__device__ __forceinline__ Parts split3(i32x8 raw) {
+  Parts s;
+#pragma unroll
+  for (int part = 0; part < 3; part++) {
+    i32x4 packed;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      packed[i] = __builtin_amdgcn_perm(raw[2 * i + 1], raw[2 * i], 0x07060302);   // the upper halves of both
+#pragma unroll
+      for (int e = 2 * i; e < 2 * i + 2; e++)
+        if (part < 2) raw[e] = (int)__float_as_uint(__uint_as_float((unsigned)raw[e]) - __uint_as_float((unsigned)raw[e] & 0xFFFF0000u));
+    }
+    s.p[part] = __builtin_bit_cast(bf16x8, packed);
+  }
+  return s;
+}
+__device__ __forceinline__ f32x16 mfma3(const Parts& w, const Parts& x, f32x16 c) {   // the small products first
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.p[2], x.p[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.p[0], x.p[2], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.p[1], x.p[1], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.p[1], x.p[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.p[0], x.p[1], c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.p[0], x.p[0], c, 0, 0, 0);
+}
+
 // Up to eight values of a row of y, one by one: residual, rounding, store.
 template <typename TO>
 __device__ __forceinline__ void put(const crnn_linear_args& a, int64_t m, int64_t n, int count, const float (&v)[8]) {
@@ -241,7 +273,8 @@ template <int N> __device__ __forceinline__ void wait_loads() {   // all but the
 
 template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST, int KG>
 __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a, int wide) {
-  typedef Slice<IN> S;
+  constexpr bool F32 = IN == CRNN_FP32;
+  typedef Slice<F32 ? CRNN_E4M3 : IN> S;   // (fp32: 32 bytes a lane, as 8 bits)
   typedef typename TypeOf<OUT>::t TO;
   constexpr int ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1, NKS = RB / S::KB, RPL = 1024 / RB;   // slices of a step, rows of a load
   constexpr int NW = 2 * WN, BM = 64 * MT, BN = 32 * WN * NT, STAGE = (BM + BN) * RB;
@@ -290,7 +323,7 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
     for (int j = 0; j < MT; j++)
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
-  typename S::frag fx[2][MT], fw[2][NT];
+  typename S::frag fx[F32 ? 1 : 2][MT], fw[F32 ? 1 : 2][NT];
   const int swz = swizzle(lane & 31);
   const unsigned char* xrow = smem + (wm * 32 * MT + (lane & 31)) * RB;
   const unsigned char* wrow = smem + BM * RB + (wn * 32 * NT + (lane & 31)) * RB;
@@ -314,13 +347,22 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
   for (int t = 0; t < nk; t += NKS == 1 ? 2 : 1) {
 #pragma unroll
     for (int u = 0; u < (NKS == 1 ? 2 : NKS); u++) {
-      const int set = u & 1, last = NKS == 1 || u == NKS - 1, step = t + (NKS == 1 ? u : 0);
+      const int set = F32 ? 0 : u & 1, last = NKS == 1 || u == NKS - 1, step = t + (NKS == 1 ? u : 0);
       const int nxt = last ? (st + 1 == NST ? 0 : st + 1) : st;
+      Parts px[F32 ? MT : 1], pw[F32 ? NT : 1];
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < NT; i++) pw[i] = split3(fw[0][i]);
+#pragma unroll
+        for (int j = 0; j < MT; j++) px[j] = split3(fx[0][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       // a matrix instruction takes 32 cycles (8 bits: 64), so what goes out between two of them costs nothing
 #pragma unroll
       for (int q = 0; q < MT * NT; q++) {
         const int i = q / MT, j = q % MT;
-        acc[i][j] = S::mfma(fw[set][i], fx[set][j], acc[i][j]);
+        if constexpr (F32) acc[i][j] = mfma3(pw[i], px[j], acc[i][j]);
+        else acc[i][j] = S::mfma(fw[set][i], fx[set][j], acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
         if (last && q == 0) {
           wait_loads<(NST - 2) * LT>();
@@ -330,7 +372,7 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
         // operands of the next slice
         constexpr int RPQ = (MT + NT + MT * NT - 1) / (MT * NT);
 #pragma unroll
-        for (int f = q * RPQ; f < (q + 1) * RPQ && f < MT + NT; f++) read(set ^ 1, nxt, last ? 0 : u + 1, f);
+        for (int f = q * RPQ; f < (q + 1) * RPQ && f < MT + NT; f++) read(F32 ? 0 : set ^ 1, nxt, last ? 0 : u + 1, f);
         // loads for NST steps on into the stage that the last barrier freed, evenly over the two slices behind it: a burst of
         // them holds the wave up (each takes the address unit, which four waves share, 16 cycles)
         constexpr int SLOTS = NKS > 1 ? 2 * MT * NT : MT * NT;
@@ -368,6 +410,35 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
         for (int j = 0; j < MT; j++)
 #pragma unroll
           for (int r = 0; r < 16; r++) acc[i][j][r] += part[(k * NW * MT * NT * 16 + (i * MT + j) * 16 + r) * 64];
+  }
+  if constexpr (F32) {
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+      for (int j = 0; j < MT; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) fine = fine && fabsf(acc[i][j][r]) < INFINITY;
+    if (!__all(fine)) {
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+          const int64_t n = n0 + wn * 32 * NT + i * 32 + (lane & 31), m = m0 + wm * 32 * MT + j * 32 + (lane & 31);
+          f32x16 t;
+#pragma unroll
+          for (int r = 0; r < 16; r++) t[r] = 0.f;
+#pragma unroll 1
+          for (int64_t k = 4 * half; k < ((a.k + 7) & ~(int64_t)7); k += 8) {   // (every lane to the same end)
+            f32x4 w = {0.f, 0.f, 0.f, 0.f}, x = w;
+            if (n < a.n && k < a.k) w = *(const f32x4*)((const float*)a.w + n * a.ldw + k);
+            if (m < a.m && k < a.k) x = *(const f32x4*)((const float*)a.x + m * a.ldx + k);
+            t = Slice<CRNN_FP32>::mfma(w, x, t);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[i][j][r] = fabsf(acc[i][j][r]) < INFINITY ? acc[i][j][r] : t[r];
+        }
+    }
   }
   constexpr int PITCH = 32 * NT * 4 + 16;
   constexpr int LPR = 4 * NT, RPI = 64 / LPR, RI = 32 / RPI;   // lanes a row, rows at a time, times
