@@ -1028,6 +1028,21 @@ __global__ __launch_bounds__(256, 2) void attention_any_kernel(const crnn_cross_
   }
 }
 
+// The blocks of one key head (its row blocks and splits, `each` of them) belong on one XCD, whose L2 then holds their keys.  Key
+// heads go round the XCDs one by one, because neighbours share their length; with too few of them to fill all XCDs evenly
+// runs of blocks are dealt instead.  -1: no block.
+__host__ __device__ __forceinline__ bool attention_deal(int64_t key_heads) { return key_heads >= 64 || key_heads % 8 == 0; }
+static int64_t attention_grid(int64_t key_heads, int64_t each) { return attention_deal(key_heads) ? (key_heads + 7) / 8 * 8 * each : (key_heads * each + 7) / 8 * 8; }
+__device__ __forceinline__ int64_t attention_block(unsigned id, int64_t key_heads, int64_t each) {
+  const int64_t xcd = id & 7, at = id >> 3;
+  if (attention_deal(key_heads)) {
+    const int64_t head = at / each * 8 + xcd;
+    return head < key_heads ? head * each + at % each : -1;
+  }
+  const int64_t total = key_heads * each, per = (total + 7) / 8, blk = xcd * per + at;
+  return blk < total && at < per ? blk : -1;
+}
+
 // Where split s of nsplit leaves row r of all rows (batch, key head, row): D unnormalised values, then (M, L) behind all of them.
 constexpr int MAX_SPLIT = 64;
 struct SplitRow {
@@ -1062,10 +1077,9 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const c
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int kw = wave / RW, rw = wave % RW;
   const int G = a.heads / a.kv_heads, D = a.head_dim;
-  const int64_t rows = a.q_len * G, nrb = (rows + 32 * RW - 1) / (32 * RW), total = a.batch * a.kv_heads * nrb * nsplit;
-  // consecutive blocks (row blocks and splits of one key head) on one XCD, whose L2 then holds their keys
-  const int64_t per = (total + 7) / 8, blk = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (blk >= total || (blockIdx.x >> 3) >= per) return;
+  const int64_t rows = a.q_len * G, nrb = (rows + 32 * RW - 1) / (32 * RW);
+  const int64_t blk = attention_block(blockIdx.x, a.batch * a.kv_heads, nrb * nsplit);
+  if (blk < 0) return;
   const int sp = (int)(blk % nsplit);
   const int64_t rb = blk / nsplit % nrb, bg = blk / nsplit / nrb, b = bg / a.kv_heads, g = bg % a.kv_heads;
   const int len = a.lengths ? max(0, (int)min((int64_t)a.lengths[b], a.kv_len)) : (int)a.kv_len;
@@ -1299,8 +1313,8 @@ __global__ __launch_bounds__(64 * KW, 2) void attention_few_kernel(const crnn_cr
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane % LPK, grp = lane / LPK;
   const int G = a.heads / a.kv_heads, D = a.head_dim, rows = (int)a.q_len * G;
-  const int64_t total = a.batch * a.kv_heads * nsplit, per = (total + 7) / 8, blk = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (blk >= total || (blockIdx.x >> 3) >= per) return;
+  const int64_t blk = attention_block(blockIdx.x, a.batch * a.kv_heads, nsplit);
+  if (blk < 0) return;
   const int sp = (int)(blk % nsplit);
   const int64_t bg = blk / nsplit, b = bg / a.kv_heads, g = bg % a.kv_heads;
   const int len = a.lengths ? max(0, (int)min((int64_t)a.lengths[b], a.kv_len)) : (int)a.kv_len;
@@ -1585,8 +1599,8 @@ int64_t cross_attention_workspace(const crnn_cross_attention_args& a) {
 template <int TYPE, int DP, int RW, int KW>
 static void attention_tile(const crnn_cross_attention_args& a, int nsplit, hipStream_t s) {
   constexpr int KT = TYPE == CRNN_BF16 && RW == 4 ? 64 : 32;
-  const int64_t rows = a.q_len * (a.heads / a.kv_heads), total = a.batch * a.kv_heads * ((rows + 32 * RW - 1) / (32 * RW)) * nsplit;
-  hipLaunchKernelGGL((attention_tile_kernel<TYPE, DP, RW, KW, KT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * RW * KW), 0, s, a, nsplit);
+  const int64_t rows = a.q_len * (a.heads / a.kv_heads), each = (rows + 32 * RW - 1) / (32 * RW) * nsplit;
+  hipLaunchKernelGGL((attention_tile_kernel<TYPE, DP, RW, KW, KT>), dim3((unsigned)attention_grid(a.batch * a.kv_heads, each)), dim3(64 * RW * KW), 0, s, a, nsplit);
 }
 template <int TYPE, int DP>
 static void attention_tile(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
@@ -1606,8 +1620,7 @@ static void attention_tile(const crnn_cross_attention_args& a, const AttnPlan& p
 template <int TYPE, int LPK, int R>
 static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
   constexpr int U = R == 4 || LPK == 4 ? 4 : 8;   // loads of each in a chunk: registers for two chunks and four rows are short
-  const int64_t total = a.batch * a.kv_heads * p.nsplit;
-  const dim3 g((unsigned)((total + 7) / 8 * 8));
+  const dim3 g((unsigned)attention_grid(a.batch * a.kv_heads, p.nsplit));
   if (p.kw == 1) hipLaunchKernelGGL((attention_few_kernel<TYPE, LPK, U, R, 1>), g, dim3(64), 0, s, a, p.nsplit);
   else hipLaunchKernelGGL((attention_few_kernel<TYPE, LPK, U, R, 4>), g, dim3(256), 0, s, a, p.nsplit);
 }
