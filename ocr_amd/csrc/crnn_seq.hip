@@ -37,13 +37,13 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// erf by Abramowitz & Stegun 7.1.26: 1 - (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p |x|), off by at most 1.5e-7 -- what
-// 1 + erf loses to rounding is of that size.  (erff and expf with a division: 94 instead of 62 + 8 us for 18176 x 512 x 2048.)
+// x Phi(x) = max(x, 0) - |x| Phi(-|x|), and Phi(-y) = erfc(y / sqrt 2) / 2 by Abramowitz & Stegun 7.1.26: (a1 t + ... + a5 t^5)
+// exp(-y^2 / 2) / 2, t = 1 / (1 + p y / sqrt 2), off by at most 0.75e-7 -- what 1 + erf loses to rounding is of that size.  (With
+// erff and expf 18176 x 512 x 2048 took 32 us more than without activation.)
 __device__ __forceinline__ float gelu(float v) {
-  const float x = fabsf(v) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  const float e = p * __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f);   // 1 - erf |x|
-  return 0.5f * v * (v > 0.f ? 2.f - e : e);
+  const float y = fabsf(v), t = __builtin_amdgcn_rcpf(fmaf(0.23164190f, y, 1.f));
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
+  return fmaf(-y, p * __builtin_amdgcn_exp2f(v * v * -0.72134752044448170f), v > 0.f ? v : 0.f);
 }
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f)); }
 __device__ __forceinline__ float activate(float v, int act) {

@@ -235,7 +235,8 @@ def qkv(g, b, t, s, heads, kvh, d, dt, spread=1.5):
 @pytest.mark.parametrize("b, t, s, heads, kvh, d", [
     (1, 1, 1, 1, 1, 1), (2, 1, 71, 8, 8, 64), (3, 5, 33, 4, 2, 32), (2, 17, 64, 2, 1, 128), (1, 130, 257, 2, 2, 64), (2, 3, 1000, 4, 4, 64), (1, 1, 5000, 8, 2, 128),
     (2, 33, 129, 3, 3, 80), (1, 7, 31, 6, 2, 17), (4, 64, 32, 1, 1, 96), (1, 1, 20000, 2, 1, 64), (1, 300, 300, 4, 1, 128), (5, 2, 2, 2, 2, 8), (2, 16, 4096, 1, 1, 40),
-    (1, 257, 65, 1, 1, 33), (3, 40, 700, 16, 1, 64)])
+    (1, 257, 65, 1, 1, 33), (3, 40, 700, 16, 1, 64), (32, 258, 400, 8, 4, 64), (16, 300, 330, 16, 8, 128), (40, 64, 300, 8, 2, 32),
+    (33, 270, 260, 8, 8, 80)])
 def test_cross_attention(crnn, b, t, s, heads, kvh, d, dt):
     g = gen(b + t + s)
     q, k, v = qkv(g, b, t, s, heads, kvh, d, dt)
