@@ -1562,7 +1562,7 @@ static bool attention_chunks(const crnn_cross_attention_args& a) {   // (sizes, 
 static bool attention_aligned(const crnn_cross_attention_args& a) { return (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0; }
 
 // How the work is cut: `rw` waves side by side over 32 rows each, or 0 for attention_few_kernel; `kw` waves over the keys;
-// nsplit workgroups over the keys where there are too few row blocks to fill the chip (512 workgroups are two per CU).
+// nsplit workgroups over the keys where there are too few row blocks to fill the chip.
 struct AttnPlan {
   int rw, kw, nsplit;
 };
@@ -1574,7 +1574,7 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
     p.rw = 0;
     p.kw = a.kv_len <= 128 && bg >= 1024 ? 1 : 4;   // few keys, many heads: a wave a head, nothing to join
     blocks = bg;
-    keys = 64 * p.kw;
+    keys = 32 * p.kw;
   } else {
     p.rw = rows > 64 ? 4 : rows > 32 ? 2 : 1;
     p.kw = a.type == CRNN_BF16 ? 4 / p.rw : p.rw == 1 ? 2 : 1;
@@ -1584,10 +1584,15 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
     keys = kt * p.kw;
   }
   const int64_t steps = (a.kv_len + keys - 1) / keys;
-  int64_t ns = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
-  if (p.rw != 0 && ns > steps / 2) ns = steps / 2;   // at least two steps each
-  if (ns > steps) ns = steps;
-  p.nsplit = (int)(ns < 1 ? 1 : ns > MAX_SPLIT ? MAX_SPLIT : ns);
+  const int64_t fill = p.rw == 0 ? 1024 : 512;                     // workgroups that fill the chip
+  int64_t ns = blocks >= fill ? 1 : (fill + blocks - 1) / blocks;
+  if (p.rw != 0 && ns > steps / 2) ns = steps / 2;                 // at least two steps each
+  if (ns > MAX_SPLIT) ns = MAX_SPLIT;
+  if (ns > 1) {                                                    // as many as the steps go into evenly
+    const int64_t per = (steps + ns - 1) / ns;
+    ns = (steps + per - 1) / per;
+  }
+  p.nsplit = (int)(ns < 1 ? 1 : ns);
   return p;
 }
 int64_t cross_attention_workspace(const crnn_cross_attention_args& a) {
@@ -1619,7 +1624,7 @@ static void attention_tile(const crnn_cross_attention_args& a, const AttnPlan& p
 }
 template <int TYPE, int LPK, int R>
 static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
-  constexpr int U = R == 4 || LPK == 4 ? 4 : 8;   // loads of each in a chunk: registers for two chunks and four rows are short
+  constexpr int U = 4;   // loads of each in a chunk (eight: a wave less per SIMD, one query over 256 lines 11.0 us for 10.4)
   const dim3 g((unsigned)attention_grid(a.batch * a.kv_heads, p.nsplit));
   if (p.kw == 1) hipLaunchKernelGGL((attention_few_kernel<TYPE, LPK, U, R, 1>), g, dim3(64), 0, s, a, p.nsplit);
   else hipLaunchKernelGGL((attention_few_kernel<TYPE, LPK, U, R, 4>), g, dim3(256), 0, s, a, p.nsplit);
