@@ -39,17 +39,27 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // x Phi(x) = max(x, 0) - |x| Phi(-|x|), and Phi(-y) = erfc(y / sqrt 2) / 2 by Abramowitz & Stegun 7.1.26: (a1 t + ... + a5 t^5)
 // exp(-y^2 / 2) / 2, t = 1 / (1 + p y / sqrt 2), off by at most 0.75e-7 -- what 1 + erf loses to rounding is of that size.  (With
-// erff and expf 18176 x 512 x 2048 took 32 us more than without activation.)
+// erff and expf 18176 x 512 x 2048 took 32 us more than without activation.)  Infinities give their limits, inf and 0,
+// because in one product 0 times infinity is 0 (v_mul_legacy_f32; a cap on |x| costs an instruction more, 4 us there).
+// (A vector instruction that reads v_rcp_f32's result waits for one state, which the compiler does not see to in assembly.)
+__device__ __forceinline__ float mul_legacy(float a, float b) {
+  float r;
+  asm("s_nop 0\n\tv_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
 __device__ __forceinline__ float gelu(float v) {
   const float y = fabsf(v), t = __builtin_amdgcn_rcpf(fmaf(0.23164190f, y, 1.f));
   const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
-  return fmaf(-y, p * __builtin_amdgcn_exp2f(v * v * -0.72134752044448170f), v > 0.f ? v : 0.f);
+  const float e = __builtin_amdgcn_exp2f(v * v * -0.72134752044448170f);
+  float yp;
+  asm("v_mul_legacy_f32 %0, |%1|, %2" : "=v"(yp) : "v"(v), "v"(p));   // (p is a product: nothing to wait for)
+  return fmaf(-yp, e, v > 0.f ? v : 0.f);
 }
-__device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f)); }
+__device__ __forceinline__ float silu(float v) { return mul_legacy(v, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f))); }
 __device__ __forceinline__ float activate(float v, int act) {
   switch (act) {
-    case CRNN_ACT_RELU: return v > 0.f ? v : 0.f;
-    case CRNN_ACT_LEAKY: return v > 0.f ? v : 0.2f * v;
+    case CRNN_ACT_RELU: return v < 0.f ? 0.f : v;   // (a NaN stays one)
+    case CRNN_ACT_LEAKY: return v < 0.f ? 0.2f * v : v;
     case CRNN_ACT_GELU: return gelu(v);
     case CRNN_ACT_SILU: return silu(v);
     default: return v;
@@ -114,7 +124,7 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
   } else if (act != CRNN_ACT_NONE) {
     const float slope = act == CRNN_ACT_LEAKY ? 0.2f : 0.f;
 #pragma unroll
-    for (int e = 0; e < N; e++) v[e] = v[e] > 0.f ? v[e] : act == CRNN_ACT_RELU ? 0.f : slope * v[e];
+    for (int e = 0; e < N; e++) v[e] = v[e] < 0.f ? (act == CRNN_ACT_RELU ? 0.f : slope * v[e]) : v[e];
   }
 }
 
@@ -712,7 +722,7 @@ static void linear_of(const crnn_linear_args& a, hipStream_t s) {
         a.m == 1 ? linear_vector<IN, OUT, 1>(a, s) : a.m == 2 ? linear_vector<IN, OUT, 2>(a, s) : linear_vector<IN, OUT, 4>(a, s);
         return;
       }
-      if (a.m <= 16 && a.n < 1 << 27) return linear_rows<IN, OUT>(a, s);
+      if (a.m <= 16 && a.n < 1 << 26) return linear_rows<IN, OUT>(a, s);
       if (linear_tiles<IN, OUT>(a, s)) return;
     }
   }

@@ -122,6 +122,20 @@ def test_linear_nan_and_infinity_stay_in_their_row_and_column(crnn, m, k, n, dt)
     assert torch.isnan(got[:, n - 1]).all() and torch.equal(got[:, :n - 1], clean[:, :n - 1])
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "e4m3"])
+@pytest.mark.parametrize("act", ["none", "relu", "leaky", "gelu", "silu"])
+def test_linear_activations_of_nan_and_infinity(crnn, act, dt):
+    """NaN stays, infinities and what overflows nothing give the limits; through each of the kernels."""
+    nan, inf = float("nan"), float("inf")
+    z = torch.tensor([nan, inf, -inf, 1e30, -1e30, 200.0, -200.0, 0.0] * 8)
+    neg = {"none": z, "leaky": 0.2 * z}.get(act, torch.zeros_like(z))
+    want = torch.where(z < 0, neg, z)
+    for m, k in ((1, 64), (3, 64), (9, 64), (40, 64), (300, 64), (700, 256), (9, 63), (300, 65)):
+        x, w = torch.zeros(m, k, device="cuda").to(DT[dt]), torch.zeros(64, k, device="cuda").to(DT[dt])
+        got = crnn.linear(x, w, bias=z.cuda(), act=act, out_dtype=torch.bfloat16)
+        torch.testing.assert_close(got.cpu(), want.to(torch.bfloat16).expand(m, 64), rtol=2.0 ** -7, atol=0, equal_nan=True, msg=lambda t: "%d x %d: %s" % (m, k, t))
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e-10, 1e10, 1e18])
 def test_linear_fp32_over_its_range(crnn, scale):
     g = gen(6)
