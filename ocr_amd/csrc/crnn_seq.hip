@@ -1564,10 +1564,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const crnn_cross_at
 
 static bool attention_chunks(const crnn_cross_attention_args& a) {   // (sizes, type and strides only)
   const int c = a.type == CRNN_BF16 ? 8 : 4;
-  if (a.head_dim % c != 0 || a.kv_len == 0) return false;
-  for (int i = 0; i < 3; i++)
-    if (a.q_stride[i] % c != 0 || a.k_stride[i] % c != 0 || a.v_stride[i] % c != 0) return false;
-  return a.k_stride[1] < (1 << 22) && a.v_stride[1] < (1 << 22);   // offsets within 64 keys stay below 2^31 bytes
+  if (a.head_dim % c != 0 || a.kv_len == 0 || a.kv_len > 0x7FF00000) return false;   // (key numbers a few steps past the end are ints)
+  const int64_t qn[3] = {a.batch, a.q_len, a.heads}, kn[3] = {a.batch, a.kv_len, a.kv_heads};
+  for (int i = 0; i < 3; i++)   // (a stride that no step is made by may be anything)
+    if ((qn[i] > 1 && a.q_stride[i] % c != 0) || (kn[i] > 1 && (a.k_stride[i] % c != 0 || a.v_stride[i] % c != 0))) return false;
+  return a.kv_len == 1 || (a.k_stride[1] < (1 << 22) && a.v_stride[1] < (1 << 22));   // offsets within 64 keys stay below 2^31 bytes
 }
 static bool attention_aligned(const crnn_cross_attention_args& a) { return (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0; }
 

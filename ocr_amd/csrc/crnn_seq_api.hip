@@ -7,7 +7,10 @@ using namespace crnn;
 
 namespace {
 
-constexpr int64_t I31 = 0x7FFFFFFF, FAR = (int64_t)1 << 40;   // strides up to FAR: no product of them passes 63 bits
+constexpr int64_t I31 = 0x7FFFFFFF, FAR = (int64_t)1 << 40;
+
+// Whether `count` steps of a stride leave what addresses can reach: offsets in bytes, sums of a few of them too, stay below 2^63.
+bool far(int64_t stride, int64_t count) { return stride < 0 || stride > FAR || (count > 1 && stride > ((int64_t)1 << 56) / count); }
 
 // [rows, cols] elements of `size` bytes, rows `ld` apart
 struct Block {
@@ -42,7 +45,7 @@ const char* check_linear(const crnn_linear_args& a) {
   if (a.m == 0) return nullptr;
   if (!a.x || !a.w || !a.y) return "crnn_linear: x, w or y is null";
   if (a.in_type != CRNN_E4M3 && (a.x_scale || a.w_scale)) return "crnn_linear: scales belong to CRNN_E4M3 operands";
-  if (a.ldx < 0 || a.ldw < 0 || a.ldr < 0 || a.ldx > FAR || a.ldw > FAR || a.ldr > FAR || a.ldy > FAR) return "crnn_linear: a row stride is out of range";
+  if (far(a.ldx, a.m) || far(a.ldw, a.n) || far(a.ldr, a.m) || far(a.ldy, a.m)) return "crnn_linear: a row stride is out of range";
   if (a.ldy < a.n && a.m > 1) return "crnn_linear: ldy is smaller than n";
   const int64_t ei = type_size(a.in_type), eo = type_size(a.out_type);
   if (!aligned(a.x, ei) || !aligned(a.w, ei) || !aligned(a.y, eo) || !aligned(a.residual, eo) || !aligned(a.bias, 4) || !aligned(a.x_scale, 4) || !aligned(a.w_scale, 4))
@@ -66,7 +69,7 @@ const char* check_norm(const crnn_rms_norm_args& a) {
   const bool e8 = a.out_type == CRNN_E4M3;
   if (!a.x || !a.gain || !a.y) return "crnn_rms_norm: x, gain or y is null";
   if (e8 != (a.y_scale != nullptr)) return "crnn_rms_norm: y_scale belongs to CRNN_E4M3 outputs, and they need it";
-  if (a.ldx < 0 || a.ldr < 0 || a.ldx > FAR || a.ldr > FAR || a.lds > FAR || a.ldy > FAR) return "crnn_rms_norm: a row stride is out of range";
+  if (far(a.ldx, a.m) || far(a.ldr, a.m) || far(a.lds, a.m) || far(a.ldy, a.m)) return "crnn_rms_norm: a row stride is out of range";
   if (a.m > 1 && (a.ldy < a.n || (a.sum && a.lds < a.n))) return "crnn_rms_norm: the rows of an output overlap";
   const int64_t ei = type_size(a.in_type), eo = type_size(a.out_type);
   if (!aligned(a.x, ei) || !aligned(a.residual, ei) || !aligned(a.sum, ei) || !aligned(a.y, eo) || !aligned(a.gain, 4) || !aligned(a.y_scale, 4))
@@ -92,13 +95,13 @@ const char* check_attention(const crnn_cross_attention_args& a, bool sizes_only)
   if (a.batch < 0 || a.q_len < 0 || a.kv_len < 0 || a.batch > I31 || a.q_len > I31 || a.kv_len > I31) return "crnn_cross_attention: batch, q_len or kv_len out of range";
   // one workgroup takes at least one row of one batch entry's key head
   if ((double)a.batch * a.heads * (double)a.q_len > 2147483647.0) return "crnn_cross_attention: batch * heads * q_len passes 2^31 - 1";
+  const int64_t qn[3] = {a.batch, a.q_len, a.heads}, kn[3] = {a.batch, a.kv_len, a.kv_heads};
   for (int i = 0; i < 3; i++)
-    if (a.q_stride[i] < 0 || a.k_stride[i] < 0 || a.v_stride[i] < 0 || a.out_stride[i] < 0 || a.q_stride[i] > FAR || a.k_stride[i] > FAR ||
-        a.v_stride[i] > FAR || a.out_stride[i] > FAR)
+    if (far(a.q_stride[i], qn[i]) || far(a.out_stride[i], qn[i]) || far(a.k_stride[i], kn[i]) || far(a.v_stride[i], kn[i]))
       return "crnn_cross_attention: a stride is out of range";
   if (sizes_only || a.batch == 0 || a.q_len == 0) return nullptr;
   if (!a.q || !a.out || (a.kv_len > 0 && (!a.k || !a.v))) return "crnn_cross_attention: q, k, v or out is null";
-  if (a.mask && (a.mask_stride < 0 || a.mask_stride > FAR)) return "crnn_cross_attention: mask_stride is out of range";
+  if (a.mask && far(a.mask_stride, a.batch)) return "crnn_cross_attention: mask_stride is out of range";
   if (!(a.scale == a.scale) || a.scale - a.scale != 0.f) return "crnn_cross_attention: scale is not finite";
   const int64_t e = type_size(a.type);
   if (!aligned(a.q, e) || !aligned(a.k, e) || !aligned(a.v, e) || !aligned(a.out, e) || !aligned(a.lengths, 4))
@@ -116,7 +119,6 @@ const char* check_attention(const crnn_cross_attention_args& a, bool sizes_only)
   for (int i = 0; i < 3; i++) {
     if (len[i] == 1) continue;
     if (st[i] < extent) return "crnn_cross_attention: rows of out overlap";
-    if ((double)st[i] * (len[i] - 1) + extent > 9e18 / e) return "crnn_cross_attention: a stride is out of range";
     extent += st[i] * (len[i] - 1);
   }
   // (inputs may be views that interleave with one another, so of them only a common address range is looked at)

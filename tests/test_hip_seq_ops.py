@@ -317,6 +317,16 @@ def test_cross_attention_strides_and_alignments(crnn, t, s, dt):
         R.check(crnn.cross_attention(q2, k, v, scale=sc), *R.attention(q2, k, v, scale=sc))
 
 
+@pytest.mark.parametrize("t, s", [(1, 1), (1, 300), (20, 1), (40, 300)])
+def test_cross_attention_strides_of_single_dimensions_do_not_matter(crnn, t, s):
+    g = gen(t + s)
+    q, k, v = randn(g, 1, t, 1, 64), randn(g, 1, s, 1, 64), randn(g, 1, s, 1, 64)
+    odd = lambda x: x.as_strided(x.shape, [3 if x.shape[i] == 1 else x.stride(i) for i in range(3)] + [1])
+    want = crnn.cross_attention(q, k, v)
+    R.check(want, *R.attention(q, k, v))
+    assert torch.equal(crnn.cross_attention(odd(q), odd(k), odd(v)), want)
+
+
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
 @pytest.mark.parametrize("t, s", [(1, 40), (1, 4000), (64, 500)])
 def test_cross_attention_scores_far_apart(crnn, t, s, dt):

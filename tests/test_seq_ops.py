@@ -34,6 +34,7 @@ LIN = dict(m=4, n=8, k=16, x=P, w=P + 4096, ldx=16, ldw=16, x_scale=None, w_scal
     (dict(act=-1), "activation"), (dict(ldy=7), "ldy"), (dict(ldx=-1), "stride"), (dict(ldw=-1), "stride"), (dict(x_scale=P + 9000), "scales"),
     (dict(x=P + 1), "aligned"), (dict(bias=P + 8193), "aligned"), (dict(y=P), "overlaps"), (dict(y=P + 4096), "overlaps"), (dict(y=P + 8192), "overlaps"),
     (dict(residual=P + 16386, ldr=8), "residual"), (dict(residual=P + 16384, ldr=9), "residual"), (dict(reserved=1), "reserved"),
+    (dict(ldx=1 << 41), "stride"), (dict(m=1 << 30, ldy=1 << 30), "stride"), (dict(n=1 << 30, ldw=1 << 40), "stride"),
     (dict(y=P + 16, ldx=24, ldy=24, n=9), "overlaps"),      # columns 8..16 of the buffer whose columns 0..15 are x
 ])
 def test_linear_refuses(handle, change, word):
@@ -52,7 +53,7 @@ NORM = dict(m=4, n=16, x=P, ldx=16, residual=P + 4096, ldr=16, gain=P + 8192, su
     (dict(eps=float("nan")), "eps"), (dict(in_type=_capi.E4M3), "in_type"), (dict(out_type=_capi.FP32), "out_type"), (dict(y_scale=P + 20000), "y_scale"),
     (dict(out_type=_capi.E4M3), "y_scale"), (dict(ldy=15), "overlap"), (dict(lds=15), "overlap"), (dict(ldx=-2), "stride"), (dict(x=P + 1), "aligned"),
     (dict(y=P + 2), "overlaps an input"), (dict(y=P, ldy=17), "overlaps an input"), (dict(sum=P + 16384), "two outputs"), (dict(y=P + 8192), "overlaps an input"),
-    (dict(reserved=7), "reserved"), (dict(out_type=_capi.E4M3, y_scale=P + 20000, y=P), "overlaps an input"),
+    (dict(m=1 << 30, ldr=1 << 40), "stride"), (dict(reserved=7), "reserved"), (dict(out_type=_capi.E4M3, y_scale=P + 20000, y=P), "overlaps an input"),
 ])
 def test_rms_norm_refuses(handle, change, word):
     lib, h = handle
@@ -73,7 +74,8 @@ ATT = dict(batch=2, q_len=3, kv_len=5, heads=4, kv_heads=2, head_dim=8, type=_ca
     (dict(q_stride=_capi.I64x3(-1, 0, 0)), "stride"), (dict(out_stride=_capi.I64x3(96, 32, 7)), "rows of out"), (dict(out_stride=_capi.I64x3(95, 32, 8)), "rows of out"),
     (dict(out_stride=_capi.I64x3(0, 32, 8)), "rows of out"), (dict(out=P), "overlaps q"), (dict(out=P + 4096), "overlaps k"), (dict(out=P + 8192), "overlaps k"),
     (dict(mask=P + 16400, mask_stride=5), "mask"), (dict(mask=P, mask_stride=-1), "mask_stride"), (dict(lengths=P + 16388), "lengths"), (dict(lengths=P + 2), "aligned"),
-    (dict(q=P + 1), "aligned"), (dict(reserved=1), "reserved"),
+    (dict(q=P + 1), "aligned"), (dict(reserved=1), "reserved"), (dict(kv_len=1 << 30, v_stride=_capi.I64x3(80, 1 << 40, 8)), "stride"),
+    (dict(q_len=1 << 20, out_stride=_capi.I64x3(96, 1 << 40, 8)), "stride"), (dict(mask=P, mask_stride=1 << 41), "mask_stride"),
 ])
 def test_cross_attention_refuses(handle, change, word):
     lib, h = handle
@@ -89,6 +91,17 @@ def test_nothing_to_do_is_no_error(handle):
     for none in (dict(batch=0), dict(q_len=0)):
         a = fields(_capi.CrossAttentionArgs, ATT, q=None, **none)
         assert lib.crnn_cross_attention(h, C.byref(a), None) == 0 and lib.crnn_cross_attention_workspace(h, C.byref(a)) == 0
+
+
+def test_workspace_is_told_from_sizes_type_and_strides(handle):
+    lib, h = handle
+    ask = lambda **c: lib.crnn_cross_attention_workspace(h, C.byref(fields(_capi.CrossAttentionArgs, ATT, **dict(dict(q=None, k=None, v=None, out=None), **c))))
+    assert ask() == 0                                               # five keys: nothing to share out
+    splits = ask(kv_len=100000) / (2 * 4 * 3 * (8 + 2) * 4)         # batch, heads, q_len; head_dim values, maximum and sum in 32 bits
+    assert splits == int(splits) and 2 <= splits <= 64
+    assert ask(kv_len=100000, k_stride=_capi.I64x3(1600000, 17, 8)) == 0      # not in whole 16 bytes: the kernel that shares nothing
+    assert ask(kv_len=(1 << 31) - 1) == 0                           # key numbers a step past these would not be ints
+    assert ask(kv_len=100000, batch=1, k_stride=_capi.I64x3(3, 16, 8)) == ask(kv_len=100000, batch=1)   # a stride that no step is made by
 
 
 def test_null_arguments(handle):
