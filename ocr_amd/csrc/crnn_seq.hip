@@ -1588,10 +1588,13 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
     keys = 32 * p.kw;
   } else {
     p.rw = rows > 64 ? 4 : rows > 32 ? 2 : 1;
-    p.kw = a.type == CRNN_BF16 ? 4 / p.rw : p.rw == 1 ? 2 : 1;
+    blocks = bg * ((rows + 32 * p.rw - 1) / (32 * p.rw));
+    // fp32 tiles take twice the LDS, so half the waves over the keys, but where at most two workgroups come to a CU: two waves
+    // of each leave SIMDs idle.  48 queries over 71 states, head_dim 64: 64 lines 18.8 us with two waves over the keys, 21.2
+    // with one; 96 lines 27.1 and 23.3.
+    p.kw = a.type == CRNN_BF16 ? 4 / p.rw : p.rw == 1 || (p.rw == 2 && blocks <= 512 && a.head_dim <= 64) ? 2 : 1;
     const int kt = a.type == CRNN_BF16 && p.rw == 4 ? 64 : 32;
     if (p.rw == 1 && a.kv_len <= 4 * kt && bg >= 1024) p.kw = 1;
-    blocks = bg * ((rows + 32 * p.rw - 1) / (32 * p.rw));
     keys = kt * p.kw;
   }
   const int64_t steps = (a.kv_len + keys - 1) / keys;
@@ -1620,10 +1623,11 @@ static void attention_tile(const crnn_cross_attention_args& a, int nsplit, hipSt
 }
 template <int TYPE, int DP>
 static void attention_tile(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
-  constexpr int K = TYPE == CRNN_BF16 ? 2 : 1;   // (fp32 tiles take twice the LDS)
+  constexpr bool B16 = TYPE == CRNN_BF16;   // (the waves over the keys are what attention_plan says)
   if (p.rw == 4) attention_tile<TYPE, DP, 4, 1>(a, p.nsplit, s);
-  else if (p.rw == 2) attention_tile<TYPE, DP, 2, K>(a, p.nsplit, s);
-  else if (p.kw > 1) attention_tile<TYPE, DP, 1, 2 * K>(a, p.nsplit, s);
+  else if (p.rw == 2 && p.kw > 1) attention_tile<TYPE, DP, 2, B16 || DP <= 64 ? 2 : 1>(a, p.nsplit, s);
+  else if (p.rw == 2) attention_tile<TYPE, DP, 2, B16 ? 2 : 1>(a, p.nsplit, s);
+  else if (p.kw > 1) attention_tile<TYPE, DP, 1, B16 ? 4 : 2>(a, p.nsplit, s);
   else attention_tile<TYPE, DP, 1, 1>(a, p.nsplit, s);
 }
 template <int TYPE>

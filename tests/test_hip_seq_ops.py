@@ -317,6 +317,22 @@ def test_cross_attention_strides_and_alignments(crnn, t, s, dt):
         R.check(crnn.cross_attention(q2, k, v, scale=sc), *R.attention(q2, k, v, scale=sc))
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("b, t, s, d", [(130, 1, 71, 64), (260, 3, 40, 24), (70, 48, 71, 64), (70, 33, 100, 32), (80, 20, 71, 64)])
+def test_cross_attention_many_lines(crnn, b, t, s, d, dt):
+    """More key heads than workgroups that fill the chip: fewer waves share the keys of one."""
+    g = gen(b + t)
+    q, k, v = qkv(g, b, t, s, 8, 8, d, dt)
+    lengths = torch.randint(0, s + 1, (b,), generator=g, device="cuda", dtype=torch.int32)
+    got = crnn.cross_attention(q, k, v, lengths=lengths)
+    some = [0, 1, b // 2, b - 1]
+    R.check(got[some], *R.attention(q[some], k[some], v[some], lengths[some]))
+    at = torch.arange(s, device="cuda") < lengths[:, None]
+    assert torch.equal(crnn.cross_attention(q, k, v, mask=at), got)          # the same keys, said another way
+    for i in range(0, b, 16):                                               # alone (other splits of the keys): the same within the bound
+        R.check(crnn.cross_attention(q[i:i + 1], k[i:i + 1], v[i:i + 1], lengths=lengths[i:i + 1]), *R.attention(q[i:i + 1], k[i:i + 1], v[i:i + 1], lengths[i:i + 1]))
+
+
 @pytest.mark.parametrize("t, s", [(1, 1), (1, 300), (20, 1), (40, 300)])
 def test_cross_attention_strides_of_single_dimensions_do_not_matter(crnn, t, s):
     g = gen(t + s)
