@@ -4,10 +4,11 @@
 #include "crnn_kernels.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace crnn {
 
-typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x2b __attribute__((ext_vector_type(2), aligned(1)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -66,38 +67,52 @@ __device__ __forceinline__ float activate(float v, int act) {
   }
 }
 
-// Eight neighbouring values of a row of whole 16-byte chunks.
-template <typename T> struct Eight;
-template <> struct Eight<float> { typedef float t __attribute__((ext_vector_type(8), aligned(16))); };
-template <> struct Eight<__bf16> { typedef __bf16 t __attribute__((ext_vector_type(8))); };
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-#pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
-}
-__device__ __forceinline__ void load8(const __bf16* p, float (&v)[8]) {
-  const bf16x8 a = *(const bf16x8*)p;
+// Eight neighbouring values of a row, at the alignment of one.
+template <typename T> struct Eight { typedef T t __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  const typename Eight<T>::t a = *(const typename Eight<T>::t*)p;
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] = (float)a[i];
 }
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  *(f32x4*)p = f32x4{v[0], v[1], v[2], v[3]};
-  *(f32x4*)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-}
-__device__ __forceinline__ void store8(__bf16* p, const float (&v)[8]) {
-  bf16x8 a;
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  typename Eight<T>::t a;
 #pragma unroll
-  for (int i = 0; i < 8; i++) a[i] = (__bf16)v[i];
-  *(bf16x8*)p = a;
+  for (int i = 0; i < 8; i++) a[i] = (T)v[i];
+  *(typename Eight<T>::t*)p = a;
 }
 __device__ __forceinline__ void store8(e4m3* p, const float (&v)[8]) {
-  i32x2 a;
+  i32x2b a;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
     a[i] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], u, true);
   }
-  *(i32x2*)p = a;
+  *(i32x2b*)p = a;
+}
+
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__bf16* p, float v) { *p = (__bf16)v; }
+__device__ __forceinline__ void store1(e4m3* p, float v) { *p = (e4m3)(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xFF); }
+// Of a row of n values those at i .. i + 7 that exist.
+template <typename T>
+__device__ __forceinline__ void part8(const T* row, int i, int n, float (&v)[8]) {
+  if (i + 8 <= n) load8(row + i, v);
+  else if (i < n) {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (i + e < n) v[e] = (float)row[i + e];
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put8(T* row, int i, int n, const float (&v)[8]) {
+  if (i + 8 <= n) store8(row + i, v);
+  else if (i < n) {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (i + e < n) store1(row + i + e, v[e]);
+  }
 }
 
 // Direct loads from memory into LDS: lane l's 16 bytes at `voff` + `soff` land at `lds` + 16 l; offsets past the resource give zeros.
@@ -125,71 +140,6 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
     const float slope = act == CRNN_ACT_LEAKY ? 0.2f : 0.f;
 #pragma unroll
     for (int e = 0; e < N; e++) v[e] = v[e] < 0.f ? (act == CRNN_ACT_RELU ? 0.f : slope * v[e]) : v[e];
-  }
-}
-
-// ---------------------------------------------------------------------------
-// linear, any strides and sizes: 64 x 64 tile of y per workgroup, four waves with 32 x 32 each; tiles of 32 values of k go
-// through LDS element by element, so nothing is asked of alignment.  x is the first operand: the 32 lanes of a half-wave
-// hold neighbouring columns of y.  8-bit values go through as bfloat16, which holds them exactly: the 8-bit matrix
-// instructions keep only 13 bits below the largest of each few products that they add first (measured: 2^8 + 2^-5 in one
-// group is exact, 2^8 + 2^-6 is 2^8; between groups and with the accumulator all 24 bits are kept).
-// ---------------------------------------------------------------------------
-template <typename TL> __device__ __forceinline__ TL load(const float* p) { return *p; }
-template <typename TL> __device__ __forceinline__ TL load(const __bf16* p) { return *p; }
-template <typename TL> __device__ __forceinline__ TL load(const e4m3* p) { return (TL)__builtin_amdgcn_cvt_f32_fp8(*p, 0); }
-
-template <int IN, int OUT>
-__global__ __launch_bounds__(256, 2) void linear_any_kernel(const crnn_linear_args a) {
-  typedef typename TypeOf<IN>::t T;
-  typedef typename TypeOf<OUT>::t TO;
-  typedef typename TypeOf<IN == CRNN_FP32 ? CRNN_FP32 : CRNN_BF16>::t TL;
-  constexpr int KT = 32, LD = IN == CRNN_FP32 ? KT + 1 : KT + 8;
-  __shared__ __attribute__((aligned(16))) TL xs[64 * LD], ws[64 * LD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int64_t ntn = (a.n + 63) / 64, tiles = (a.m + 63) / 64 * ntn;
-  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-  const T* x = (const T*)a.x;
-  const T* w = (const T*)a.w;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int64_t m0 = tile / ntn * 64, n0 = tile % ntn * 64;
-    f32x16 acc;
-#pragma unroll
-    for (int r = 0; r < 16; r++) acc[r] = 0.f;
-    for (int64_t k0 = 0; k0 < a.k; k0 += KT) {
-#pragma unroll
-      for (int i = 0; i < 64 * KT / 256; i++) {
-        const int e = tid + 256 * i, row = e / KT, c = e % KT;
-        const bool kin = k0 + c < a.k;
-        xs[row * LD + c] = kin && m0 + row < a.m ? load<TL>(x + (m0 + row) * a.ldx + k0 + c) : (TL)0;
-        ws[row * LD + c] = kin && n0 + row < a.n ? load<TL>(w + (n0 + row) * a.ldw + k0 + c) : (TL)0;
-      }
-      __syncthreads();
-      const TL* xr = xs + (wm + (lane & 31)) * LD;
-      const TL* wr = ws + (wn + (lane & 31)) * LD;
-      if constexpr (IN != CRNN_FP32) {
-#pragma unroll
-        for (int c = 0; c < KT; c += 16)
-          acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(xr + c + 8 * half), *(const bf16x8*)(wr + c + 8 * half), acc, 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int c = 0; c < KT; c += 2) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(xr[c + half], wr[c + half], acc, 0, 0, 0);
-      }
-      __syncthreads();
-    }
-    const int64_t n = n0 + wn + (lane & 31);
-    if (n >= a.n) continue;
-    const float ws1 = a.w_scale ? a.w_scale[n] : 1.f, b = a.bias ? a.bias[n] : 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; r++) {
-      const int64_t m = m0 + wm + acc_row(r, lane);
-      if (m >= a.m) continue;
-      float v = acc[r];
-      if (IN == CRNN_E4M3) v = v * (a.x_scale ? a.x_scale[m] : 1.f) * ws1;
-      v = activate(v + b, a.act);
-      if (a.residual) v += (float)((const TO*)a.residual)[m * a.ldr + n];
-      ((TO*)a.y)[m * a.ldy + n] = (TO)v;
-    }
   }
 }
 
@@ -266,6 +216,37 @@ __device__ __forceinline__ f32x16 mfma3(const Parts& w, const Parts& x, f32x16 c
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.p[0], x.p[0], c, 0, 0, 0);
 }
 
+// Results of the three-part products that are not finite, again on the f32 instructions: sums of a wave's 32 MT x 32 NT part of y
+// whose first row and column are m0, n0.
+template <int MT, int NT>
+__device__ __forceinline__ void finite_sums(const crnn_linear_args& a, f32x16 (&acc)[NT][MT], int64_t m0, int64_t n0, int lane) {
+  bool fine = true;
+#pragma unroll
+  for (int i = 0; i < NT; i++)
+#pragma unroll
+    for (int j = 0; j < MT; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) fine = fine && fabsf(acc[i][j][r]) < INFINITY;
+  if (__all(fine)) return;
+#pragma unroll
+  for (int i = 0; i < NT; i++)
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+      const int64_t n = n0 + i * 32 + (lane & 31), m = m0 + j * 32 + (lane & 31);
+      f32x16 t;
+#pragma unroll
+      for (int r = 0; r < 16; r++) t[r] = 0.f;
+#pragma unroll 4
+      for (int64_t k = lane >> 5; k < ((a.k + 1) & ~(int64_t)1); k += 2) {   // (every lane to the same end)
+        const float w = n < a.n && k < a.k ? ((const float*)a.w)[n * a.ldw + k] : 0.f;
+        const float x = m < a.m && k < a.k ? ((const float*)a.x)[m * a.ldx + k] : 0.f;
+        t = __builtin_amdgcn_mfma_f32_32x32x2f32(w, x, t, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = fabsf(acc[i][j][r]) < INFINITY ? acc[i][j][r] : t[r];
+    }
+}
+
 // Up to eight values of a row of y, one by one: residual, rounding, store.
 template <typename TO>
 __device__ __forceinline__ void put(const crnn_linear_args& a, int64_t m, int64_t n, int count, const float (&v)[8]) {
@@ -276,13 +257,258 @@ __device__ __forceinline__ void put(const crnn_linear_args& a, int64_t m, int64_
     if (i < count) y[i] = (TO)(r ? v[i] + (float)r[i] : v[i]);
 }
 
+// The sums of a wave's 32 MT x 32 NT part of y become y: 32 rows at a time go through LDS (4096 NT bytes of the wave's own at
+// `ex`; 16-byte chunk c of row r at c ^ swizzle(r)), after which a lane holds eight neighbours of a row: bias, activation and
+// residual happen there, and rows leave as whole lines, 16 bytes a lane at whatever alignment the rows have.  m0, n0: the
+// part's first row and column.
+template <int IN, int OUT, int MT, int NT>
+__device__ __forceinline__ void linear_out(const crnn_linear_args& a, f32x16 (&acc)[NT][MT], unsigned char* ex, int64_t m0, int64_t n0, int lane) {
+  typedef typename TypeOf<OUT>::t TO;
+  typedef typename Eight<TO>::t E8;
+  constexpr int LPR = 4 * NT, RPI = 64 / LPR, RI = 32 / RPI;   // lanes a row, rows at a time, times
+  auto swizzle = [](int r) { return NT == 1 ? (r >> 1) & 7 : r & 15; };
+  const int half = lane >> 5, c = lane % LPR;
+  const int64_t n = n0 + c * 8, left = a.n - n, mw = m0 + lane / LPR;   // this lane's rows: mw + 32 j + RPI i
+  float bias[8], wsc[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    bias[e] = a.bias && e < left ? a.bias[n + e] : 0.f;
+    wsc[e] = IN == CRNN_E4M3 && a.w_scale && e < left ? a.w_scale[n + e] : 1.f;
+  }
+  // the residual of the next 32 rows (fp32: of these, registers are short) is on its way while these are worked on
+  constexpr int AHEAD = sizeof(TO) == 2;
+  E8 res[1 + AHEAD][RI];
+  auto fetch = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < RI; i++) {
+      const int64_t m = mw + 32 * j + RPI * i;
+      if (a.residual && left >= 8 && m < a.m) res[j & AHEAD][i] = *(const E8*)((const TO*)a.residual + m * a.ldr + n);
+    }
+  };
+  if (AHEAD) fetch(0);
+#pragma unroll
+  for (int j = 0; j < MT; j++) {
+    const int r = lane & 31;
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+      for (int g = 0; g < 4; g++)
+        *(f32x4*)(ex + r * 128 * NT + (((8 * i + 2 * g + half) ^ swizzle(r)) << 4)) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+    if (j + AHEAD < MT) fetch(j + AHEAD);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    float v[8 * RI];
+#pragma unroll
+    for (int i = 0; i < RI; i++) {
+      const int r = lane / LPR + RPI * i;
+      const f32x4 lo = *(const f32x4*)(ex + r * 128 * NT + (((2 * c) ^ swizzle(r)) << 4)), hi = *(const f32x4*)(ex + r * 128 * NT + (((2 * c + 1) ^ swizzle(r)) << 4));
+      float sx = 1.f;
+      if (IN == CRNN_E4M3 && a.x_scale && mw + 32 * j + RPI * i < a.m) sx = a.x_scale[mw + 32 * j + RPI * i];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float u = e < 4 ? lo[e & 3] : hi[e & 3];
+        v[8 * i + e] = IN == CRNN_E4M3 ? u * sx * wsc[e] + bias[e] : u + bias[e];
+      }
+    }
+    activate_all(v, a.act);
+#pragma unroll
+    for (int i = 0; i < RI; i++) {
+      const int64_t m = mw + 32 * j + RPI * i;
+      float u[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) u[e] = v[8 * i + e];
+      if (m >= a.m || left <= 0) continue;
+      if (left < 8) {
+        put<TO>(a, m, n, (int)left, u);
+        continue;
+      }
+      E8 y;
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = (TO)(a.residual ? u[e] + (float)res[j & AHEAD][i][e] : u[e]);
+      *(E8*)((TO*)a.y + m * a.ldy + n) = y;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// EPC neighbours of a row of k values from k0 on, at the alignment of one value; zeros past the end.  A chunk that the end cuts is
+// read from where it ends with the row, and moved down.
+template <typename T, int EPC> struct Chunk {
+  typedef int raw __attribute__((ext_vector_type(EPC * sizeof(T) / 4)));
+  typedef int raw_at __attribute__((ext_vector_type(EPC * sizeof(T) / 4), aligned(sizeof(T))));
+  static __device__ __forceinline__ raw whole(const T* p) { return *(const raw_at*)p; }
+  static __device__ __forceinline__ raw any(const T* row, int64_t k0, int64_t k) {
+    raw v = {};
+    if (k0 >= k) return v;
+    if (k0 + EPC <= k) return whole(row + k0);
+    typedef typename std::conditional<sizeof(raw) == 16, unsigned __int128, unsigned long long>::type bits;
+    if (k >= EPC) return __builtin_bit_cast(raw, __builtin_bit_cast(bits, whole(row + k - EPC)) >> (int)((k0 - (k - EPC)) * sizeof(T) * 8));
+    bits b = 0;
+#pragma unroll
+    for (int e = EPC - 1; e >= 0; e--) {
+      typedef typename std::conditional<sizeof(T) == 4, unsigned, typename std::conditional<sizeof(T) == 2, unsigned short, unsigned char>::type>::type word;
+      b = (b << (sizeof(T) * 8)) | (k0 + e < k ? ((const word*)row)[k0 + e] : 0);
+    }
+    return __builtin_bit_cast(raw, b);
+  }
+  // `row` exists or the chunk is zeros; `inside`: it ends before k, for every lane
+  static __device__ __forceinline__ raw get(const T* row, int64_t k0, int64_t k, bool exists, bool inside) {
+    raw v = {};
+    if (exists) v = inside ? whole(row + k0) : any(row, k0, k);
+    return v;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// linear, any strides, alignments and sizes: as linear_tile_kernel with 32 MT x 32 NT a wave, 2 x 2 waves, but operands go to LDS
+// through registers, because loads straight to LDS want whole 16-byte chunks: a step's loads are on their way while the step
+// before is multiplied.  8-bit values become bfloat16 on the way, which holds them exactly: the 8-bit matrix instructions keep
+// only 13 bits below the largest of each few products that they add first (measured: 2^8 + 2^-5 in one group is exact,
+// 2^8 + 2^-6 is 2^8; between groups and with the accumulator all 24 bits are kept), too few for results in 32 bits.
+// ---------------------------------------------------------------------------
+template <int IN, int OUT, int MT, int NT, int KG>
+__global__ __launch_bounds__(256 * KG, 2) void linear_loose_kernel(const crnn_linear_args a) {
+  typedef typename TypeOf<IN>::t T;
+  constexpr bool F32 = IN == CRNN_FP32;
+  typedef Slice<F32 ? CRNN_E4M3 : CRNN_BF16> S;   // (fp32: 32 bytes a lane)
+  constexpr int RB = 128, NKS = RB / S::KB, KE = F32 ? 32 : 64, EPC = KE / 8;   // bytes of a row of a step in LDS, slices, values, of a chunk
+  constexpr int BM = 64 * MT, BN = 64 * NT, STAGE = (BM + BN) * RB, CH = (BM + BN) / 32;   // chunks of a thread and step
+  constexpr int JOIN = (KG - 1) * 4 * MT * NT * 4096;   // bytes of the other groups' sums
+  __shared__ __attribute__((aligned(1024))) unsigned char smem_all[KG * 2 * STAGE];
+  static_assert(sizeof(smem_all) >= JOIN + 4 * 4096 * NT, "the epilogue's exchange fits");
+  typedef Chunk<T, EPC> C;
+  const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wm = wave >> 1, wn = wave & 1;
+  unsigned char* smem = smem_all + kg * 2 * STAGE;
+  auto swizzle = [](int r) { return (r >> 1) & 7; };
+  const int64_t ntm = (a.m + BM - 1) / BM, ntn = (a.n + BN - 1) / BN, total = ntm * ntn, per = (total + 7) / 8;
+  const int64_t nk = (a.k + KE * KG - 1) / (KE * KG);   // steps of a group: KG t + kg
+  for (int64_t at = blockIdx.x >> 3; at < per; at += gridDim.x >> 3) {   // (the order of linear_tile_kernel)
+    const int64_t t0 = (blockIdx.x & 7) * per + at;
+    if (t0 >= total) break;
+    const int64_t grp = t0 / (8 * ntn), in = t0 - grp * 8 * ntn, gm = min((int64_t)8, ntm - grp * 8);
+    const int64_t m0 = (grp * 8 + in % gm) * BM, n0 = in / gm * BN;
+    typename C::raw st[CH];
+    auto fetch = [&](int64_t step) __attribute__((always_inline)) {
+      const int64_t ks = (step * KG + kg) * KE, k0 = ks + (tid & 7) * EPC;
+      const bool inside = ks + KE <= a.k;   // (the same for all)
+#pragma unroll
+      for (int i = 0; i < CH; i++) {
+        const int r = (tid >> 3) + 32 * i;   // 32 i below BM: a row of x
+        const bool isx = 32 * i < BM;
+        const int64_t row = isx ? m0 + r : n0 + r - BM;
+        const T* p = isx ? (const T*)a.x + row * a.ldx : (const T*)a.w + row * a.ldw;
+        st[i] = C::get(p, k0, a.k, row < (isx ? a.m : a.n), inside);
+      }
+    };
+    auto put_stage = [&](int stage) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < CH; i++) {
+        const int r = (tid >> 3) + 32 * i;
+        i32x4 v;
+        if constexpr (IN == CRNN_E4M3) {
+          bf16x8 b;
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            b[4 * e] = (__bf16)__builtin_amdgcn_cvt_f32_fp8(st[i][e], 0), b[4 * e + 1] = (__bf16)__builtin_amdgcn_cvt_f32_fp8(st[i][e], 1),
+            b[4 * e + 2] = (__bf16)__builtin_amdgcn_cvt_f32_fp8(st[i][e], 2), b[4 * e + 3] = (__bf16)__builtin_amdgcn_cvt_f32_fp8(st[i][e], 3);
+          v = __builtin_bit_cast(i32x4, b);
+        } else {
+          v = st[i];
+        }
+        *(i32x4*)(smem + stage * STAGE + r * RB + (((tid & 7) ^ swizzle(r)) << 4)) = v;
+      }
+    };
+    auto meet = []() __attribute__((always_inline)) {   // LDS writes and reads done, of everybody; loads stay on their way
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+    f32x16 acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+      for (int j = 0; j < MT; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+    fetch(0);
+    put_stage(0);
+    fetch(1);
+    meet();
+    const int swz = swizzle(lane & 31);
+    const unsigned char* xrow = smem + (wm * 32 * MT + (lane & 31)) * RB;
+    const unsigned char* wrow = smem + BM * RB + (wn * 32 * NT + (lane & 31)) * RB;
+#pragma unroll 1
+    for (int64_t t = 0; t < nk; t++) {
+      const int stage = (int)(t & 1);
+#pragma unroll
+      for (int ks = 0; ks < NKS; ks++) {
+        typename S::frag fx[MT], fw[NT];
+#pragma unroll
+        for (int i = 0; i < NT; i++) fw[i] = S::read(wrow + stage * STAGE + i * 32 * RB, ks, half, swz);
+#pragma unroll
+        for (int j = 0; j < MT; j++) fx[j] = S::read(xrow + stage * STAGE + j * 32 * RB, ks, half, swz);
+        if constexpr (F32) {
+          Parts px[MT], pw[NT];
+#pragma unroll
+          for (int i = 0; i < NT; i++) pw[i] = split3(fw[i]);
+#pragma unroll
+          for (int j = 0; j < MT; j++) px[j] = split3(fx[j]);
+#pragma unroll
+          for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int j = 0; j < MT; j++) acc[i][j] = mfma3(pw[i], px[j], acc[i][j]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int j = 0; j < MT; j++) acc[i][j] = S::mfma(fw[i], fx[j], acc[i][j]);
+        }
+      }
+      if (t + 1 < nk) {
+        put_stage(stage ^ 1);
+        if (t + 2 < nk) fetch(t + 2);
+      }
+      meet();
+    }
+    if constexpr (KG > 1) {   // the groups' sums, added in their order
+      float* part = (float*)smem_all + (wave * MT * NT * 16) * 64 + lane;
+      if (kg > 0) {
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+          for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) part[((kg - 1) * 4 * MT * NT * 16 + (i * MT + j) * 16 + r) * 64] = acc[i][j][r];
+      }
+      meet();
+      if (kg == 0) {
+#pragma unroll
+        for (int k = 0; k < KG - 1; k++)
+#pragma unroll
+          for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int j = 0; j < MT; j++)
+#pragma unroll
+              for (int r = 0; r < 16; r++) acc[i][j][r] += part[(k * 4 * MT * NT * 16 + (i * MT + j) * 16 + r) * 64];
+      }
+    }
+    if (kg == 0) {
+      if constexpr (F32) finite_sums<MT, NT>(a, acc, m0 + wm * 32 * MT, n0 + wn * 32 * NT, lane);
+      linear_out<IN, OUT, MT, NT>(a, acc, smem_all + JOIN + wave * 4096 * NT, m0 + wm * 32 * MT, n0 + wn * 32 * NT, lane);
+    }
+    meet();   // (the next tile's operands)
+  }
+}
+
 template <int N> __device__ __forceinline__ void wait_loads() {   // all but the last N loads have landed; LDS reads done
   static_assert(N < 64, "vmcnt has six bits");
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST, int KG>
-__global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a, int wide) {
+__global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a) {
   constexpr bool F32 = IN == CRNN_FP32;
   typedef Slice<F32 ? CRNN_E4M3 : IN> S;   // (fp32: 32 bytes a lane, as 8 bits)
   typedef typename TypeOf<OUT>::t TO;
@@ -291,7 +517,7 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
   constexpr int LX = BM / (RPL * NW), LT = (BM + BN) / (RPL * NW);   // dma16 instructions of a wave and step: of x, all
   constexpr int JOIN = (KG - 1) * NW * MT * NT * 4096;   // bytes of the other groups' sums
   __shared__ __attribute__((aligned(1024))) unsigned char smem_all[KG * NST * STAGE];
-  static_assert(sizeof(smem_all) >= JOIN + NW * 32 * (32 * NT * 4 + 16), "the epilogue's exchange fits");
+  static_assert(sizeof(smem_all) >= JOIN + NW * 4096 * NT, "the epilogue's exchange fits");
   if constexpr (MT * NT > 8) CRNN_WHOLE_REGISTER_FILE();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, half = lane >> 5;
   const int kg = __builtin_amdgcn_readfirstlane(tid >> 6) / NW;
@@ -422,103 +648,9 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
           for (int r = 0; r < 16; r++) acc[i][j][r] += part[(k * NW * MT * NT * 16 + (i * MT + j) * 16 + r) * 64];
   }
   if constexpr (F32) {
-    bool fine = true;
-#pragma unroll
-    for (int i = 0; i < NT; i++)
-#pragma unroll
-      for (int j = 0; j < MT; j++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) fine = fine && fabsf(acc[i][j][r]) < INFINITY;
-    if (!__all(fine)) {
-#pragma unroll
-      for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int j = 0; j < MT; j++) {
-          const int64_t n = n0 + wn * 32 * NT + i * 32 + (lane & 31), m = m0 + wm * 32 * MT + j * 32 + (lane & 31);
-          f32x16 t;
-#pragma unroll
-          for (int r = 0; r < 16; r++) t[r] = 0.f;
-#pragma unroll 1
-          for (int64_t k = 4 * half; k < ((a.k + 7) & ~(int64_t)7); k += 8) {   // (every lane to the same end)
-            f32x4 w = {0.f, 0.f, 0.f, 0.f}, x = w;
-            if (n < a.n && k < a.k) w = *(const f32x4*)((const float*)a.w + n * a.ldw + k);
-            if (m < a.m && k < a.k) x = *(const f32x4*)((const float*)a.x + m * a.ldx + k);
-            t = Slice<CRNN_FP32>::mfma(w, x, t);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; r++) acc[i][j][r] = fabsf(acc[i][j][r]) < INFINITY ? acc[i][j][r] : t[r];
-        }
-    }
+    finite_sums<MT, NT>(a, acc, m0 + wm * 32 * MT, n0 + wn * 32 * NT, lane);
   }
-  constexpr int PITCH = 32 * NT * 4 + 16;
-  constexpr int LPR = 4 * NT, RPI = 64 / LPR, RI = 32 / RPI;   // lanes a row, rows at a time, times
-  unsigned char* ex = smem_all + JOIN + wave * 32 * PITCH;
-  const int c = (lane % LPR) * 8;
-  const int64_t n = n0 + wn * 32 * NT + c, left = a.n - n;
-  const int64_t mw = m0 + wm * 32 * MT + lane / LPR;   // this lane's rows: mw + 32 j + RPI i
-  const bool vec = wide && left >= 8;
-  float bias[8], wsc[8];
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-    bias[e] = a.bias && e < left ? a.bias[n + e] : 0.f;
-    wsc[e] = IN == CRNN_E4M3 && a.w_scale && e < left ? a.w_scale[n + e] : 1.f;
-  }
-  // the residual of the next 32 rows (fp32: of these, registers are short) is on its way while these are worked on
-  typedef typename Eight<TO>::t E8;
-  constexpr int AHEAD = sizeof(TO) == 2;
-  E8 res[1 + AHEAD][RI];
-  auto fetch = [&](int j) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < RI; i++) {
-      const int64_t m = mw + 32 * j + RPI * i;
-      if (a.residual && vec && m < a.m) res[j & AHEAD][i] = *(const E8*)((const TO*)a.residual + m * a.ldr + n);
-    }
-  };
-  if (AHEAD) fetch(0);
-#pragma unroll
-  for (int j = 0; j < MT; j++) {
-#pragma unroll
-    for (int i = 0; i < NT; i++)
-#pragma unroll
-      for (int g = 0; g < 4; g++)
-        *(f32x4*)(ex + (lane & 31) * PITCH + (i * 32 + 8 * g + 4 * half) * 4) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-    if (j + AHEAD < MT) fetch(j + AHEAD);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
-    float v[8 * RI];
-#pragma unroll
-    for (int i = 0; i < RI; i++) {
-      const int r = lane / LPR + RPI * i;
-      const f32x4 lo = *(const f32x4*)(ex + r * PITCH + c * 4), hi = *(const f32x4*)(ex + r * PITCH + c * 4 + 16);
-      float sx = 1.f;
-      if (IN == CRNN_E4M3 && a.x_scale && mw + 32 * j + RPI * i < a.m) sx = a.x_scale[mw + 32 * j + RPI * i];
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float u = e < 4 ? lo[e & 3] : hi[e & 3];
-        v[8 * i + e] = IN == CRNN_E4M3 ? u * sx * wsc[e] + bias[e] : u + bias[e];
-      }
-    }
-    activate_all(v, a.act);
-#pragma unroll
-    for (int i = 0; i < RI; i++) {
-      const int64_t m = mw + 32 * j + RPI * i;
-      float u[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) u[e] = v[8 * i + e];
-      if (m >= a.m || left <= 0) continue;
-      if (!vec) {
-        put<TO>(a, m, n, left < 8 ? (int)left : 8, u);
-        continue;
-      }
-      if (a.residual) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) u[e] += (float)res[j & AHEAD][i][e];
-      }
-      store8((TO*)a.y + m * a.ldy + n, u);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
-  }
+  linear_out<IN, OUT, MT, NT>(a, acc, smem_all + JOIN + wave * 4096 * NT, m0 + wm * 32 * MT, n0 + wn * 32 * NT, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -594,7 +726,7 @@ __global__ __launch_bounds__(64 * KW, 2) void linear_rows_kernel(const crnn_line
 
 // One to four rows: a wave per NC columns of y, its lanes side by side along k, 16 bytes of every column and row each; fp32 FMAs.
 // Nothing but the first bytes' way and the reading of w: four loads of each column are on their way at a time.
-template <int IN, int OUT, int M, int NC>
+template <int IN, int OUT, int M, int NC, bool CHUNKS>
 __global__ __launch_bounds__(256, 2) void linear_vector_kernel(const crnn_linear_args a) {
   typedef typename TypeOf<IN>::t T;
   typedef typename TypeOf<OUT>::t TO;
@@ -624,10 +756,17 @@ __global__ __launch_bounds__(256, 2) void linear_vector_kernel(const crnn_linear
     for (int u = 0; u < U; u++) {
       const unsigned kb = k0 + u * 1024;
       const bool in = kb < kbytes;
+      if constexpr (CHUNKS) {
 #pragma unroll
-      for (int c = 0; c < NC; c++) w[u][c] = __builtin_amdgcn_raw_buffer_load_b128(rw, in && n0 + c < a.n ? (unsigned)(c * (int)a.ldw * ES) + kb : OUTSIDE, 0, 0);
+        for (int c = 0; c < NC; c++) w[u][c] = __builtin_amdgcn_raw_buffer_load_b128(rw, in && n0 + c < a.n ? (unsigned)(c * (int)a.ldw * ES) + kb : OUTSIDE, 0, 0);
 #pragma unroll
-      for (int m = 0; m < M; m++) x[u][m] = __builtin_amdgcn_raw_buffer_load_b128(rx, in && m < a.m ? (unsigned)(m * (int)a.ldx * ES) + kb : OUTSIDE, 0, 0);
+        for (int m = 0; m < M; m++) x[u][m] = __builtin_amdgcn_raw_buffer_load_b128(rx, in && m < a.m ? (unsigned)(m * (int)a.ldx * ES) + kb : OUTSIDE, 0, 0);
+      } else {
+#pragma unroll
+        for (int c = 0; c < NC; c++) w[u][c] = Chunk<T, EPC>::get((const T*)a.w + (n0 + c) * a.ldw, kb / ES, a.k, n0 + c < a.n, kb - lane * 16 + 1024 <= kbytes);
+#pragma unroll
+        for (int m = 0; m < M; m++) x[u][m] = Chunk<T, EPC>::get((const T*)a.x + m * a.ldx, kb / ES, a.k, m < a.m, kb - lane * 16 + 1024 <= kbytes);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -667,18 +806,14 @@ __global__ __launch_bounds__(256, 2) void linear_vector_kernel(const crnn_linear
 // Rows of whole 16-byte chunks, and offsets within a tile below 2^31 bytes.
 static bool linear_chunks(const crnn_linear_args& a) {
   const int64_t es = a.in_type == CRNN_FP32 ? 4 : a.in_type == CRNN_BF16 ? 2 : 1, c = 16 / es;
-  if (a.in_type == CRNN_E4M3 && a.out_type == CRNN_FP32) return false;
   return a.k % c == 0 && a.ldx % c == 0 && a.ldw % c == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 &&
          (256 * (a.ldx > a.ldw ? a.ldx : a.ldw) + a.k) * es < 0x7FFFF000;
 }
 
 template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST, int KG = 1>
 static void linear_tile(const crnn_linear_args& a, hipStream_t s) {
-  const int64_t eo = OUT == CRNN_FP32 ? 4 : 2;
-  auto chunks = [&](const void* p, int64_t ld) { return (((uintptr_t)p | (uintptr_t)(ld * eo)) & 15) == 0; };
-  const int wide = chunks(a.y, a.ldy) && (!a.residual || chunks(a.residual, a.ldr));
   const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 32 * WN * NT - 1) / (32 * WN * NT));
-  hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT, WN, RB, NST, KG>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(128 * WN * KG), 0, s, a, wide);
+  hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT, WN, RB, NST, KG>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(128 * WN * KG), 0, s, a);
 }
 template <int IN, int OUT>
 static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
@@ -707,26 +842,37 @@ static void linear_rows(const crnn_linear_args& a, hipStream_t s) {
   else if (a.k * ES <= 4096) hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, 8>), g, dim3(512), 0, s, a);
   else hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, 16>), g, dim3(1024), 0, s, a);
 }
-template <int IN, int OUT, int M>
+template <int IN, int OUT, int M, bool CHUNKS>
 static void linear_vector(const crnn_linear_args& a, hipStream_t s) {
   // (a wave for one column while that does not fill the chip four times over)
-  if (a.n <= 4096) hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 1>), dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 4>), dim3((unsigned)((a.n + 15) / 16)), dim3(256), 0, s, a);
+  if (a.n <= 4096) hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 1, CHUNKS>), dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 4, CHUNKS>), dim3((unsigned)((a.n + 15) / 16)), dim3(256), 0, s, a);
+}
+template <int IN, int OUT, bool CHUNKS>
+static void linear_vector(const crnn_linear_args& a, hipStream_t s) {
+  if (a.m == 1) linear_vector<IN, OUT, 1, CHUNKS>(a, s);
+  else if (a.m == 2) linear_vector<IN, OUT, 2, CHUNKS>(a, s);
+  else linear_vector<IN, OUT, 4, CHUNKS>(a, s);
+}
+template <int IN, int OUT, int MT, int KG>
+static void linear_loose(const crnn_linear_args& a, hipStream_t s) {
+  const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 64 * MT - 1) / (64 * MT));
+  hipLaunchKernelGGL((linear_loose_kernel<IN, OUT, MT, MT, KG>), dim3((unsigned)(total < (1 << 20) ? (total + 7) / 8 * 8 : 1 << 20)), dim3(256 * KG), 0, s, a);
 }
 
 template <int IN, int OUT>
 static void linear_of(const crnn_linear_args& a, hipStream_t s) {
+  const bool chunks = linear_chunks(a);
+  const bool few = a.n < 1 << 26 && a.k < 1 << 28;   // (a launch has fewer than 2^32 threads; places in a row are 32-bit)
+  if (a.m <= 4 && few) return chunks ? linear_vector<IN, OUT, true>(a, s) : linear_vector<IN, OUT, false>(a, s);
   if constexpr (IN != CRNN_E4M3 || OUT == CRNN_BF16) {
-    if (linear_chunks(a)) {
-      if (a.m <= 4 && a.n < 1 << 26) {
-        a.m == 1 ? linear_vector<IN, OUT, 1>(a, s) : a.m == 2 ? linear_vector<IN, OUT, 2>(a, s) : linear_vector<IN, OUT, 4>(a, s);
-        return;
-      }
-      if (a.m <= 16 && a.n < 1 << 26) return linear_rows<IN, OUT>(a, s);
-      if (linear_tiles<IN, OUT>(a, s)) return;
-    }
+    if (chunks && a.m <= 16 && few) return linear_rows<IN, OUT>(a, s);
+    if (chunks && linear_tiles<IN, OUT>(a, s)) return;
   }
-  hipLaunchKernelGGL((linear_any_kernel<IN, OUT>), grid_for((a.m + 63) / 64 * ((a.n + 63) / 64)), dim3(256), 0, s, a);
+  const int64_t small = ((a.m + 127) / 128) * ((a.n + 127) / 128), tiny = ((a.m + 63) / 64) * ((a.n + 63) / 64);
+  if (small >= 256) linear_loose<IN, OUT, 2, 1>(a, s);
+  else if (tiny <= 256) linear_loose<IN, OUT, 1, 2>(a, s);
+  else linear_loose<IN, OUT, 1, 1>(a, s);
 }
 
 void launch_linear(const crnn_linear_args& a, hipStream_t s) {
@@ -766,7 +912,6 @@ __device__ __forceinline__ float row_scale(unsigned top) {
   const float t = __uint_as_float(top), low = 448.f * 0x1p-126f;   // (a row of zeros: a scale that divides)
   return (t < low ? low : t) / 448.f;
 }
-__device__ __forceinline__ e4m3 to_e4m3(float v) { return (e4m3)(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xFF); }
 
 // Sum over the 64 or 256 threads of a row (256: through LDS, between barriers).
 template <int TPR, typename V> __device__ __forceinline__ V row_sum(V v, V* part) {
@@ -827,8 +972,7 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(const crnn_rms_norm_a
     for (int64_t i = tid; i < a.n; i += 256) {
       const float t = value(i), y = t * r1 * r2 * a.gain[i];
       if (a.sum) ((T*)a.sum)[m * a.lds + i] = (T)t;
-      if constexpr (OUT == CRNN_E4M3) ((e4m3*)a.y)[m * a.ldy + i] = to_e4m3(y * ic);
-      else ((TO*)a.y)[m * a.ldy + i] = (TO)y;
+      store1((TO*)a.y + m * a.ldy + i, OUT == CRNN_E4M3 ? y * ic : y);
     }
     if (OUT == CRNN_E4M3 && tid == 0) a.y_scale[m] = c;
     __syncthreads();   // (part)
@@ -853,10 +997,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args 
     const int i = (c * TPR + at) * 8;
 #pragma unroll
     for (int e = 0; e < 8; e++) g[c][e] = 0.f;
-    if (i < n) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) g[c][e] = a.gain[i + e];
-    }
+    part8(a.gain, i, n, g[c]);
   }
   // (TPR 256: every thread of the workgroup has the same row, so the barriers in row_sum are met by all)
   for (int64_t m = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; m < a.m; m += (int64_t)gridDim.x * RPB) {
@@ -868,14 +1009,12 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args 
       const int i = (c * TPR + at) * 8;
 #pragma unroll
       for (int e = 0; e < 8; e++) t[c][e] = 0.f;
-      if (i < n) {
-        load8(x + i, t[c]);
-        if (a.residual) {
-          float r[8];
-          load8(res + i, r);
+      part8(x, i, n, t[c]);
+      if (a.residual) {
+        float r[8] = {};
+        part8(res, i, n, r);
 #pragma unroll
-          for (int e = 0; e < 8; e++) t[c][e] += r[e];
-        }
+        for (int e = 0; e < 8; e++) t[c][e] += r[e];
       }
     }
 #pragma unroll
@@ -895,10 +1034,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args 
     }
     if (a.sum) {
 #pragma unroll
-      for (int c = 0; c < C; c++) {
-        const int i = (c * TPR + at) * 8;
-        if (i < n) store8((T*)a.sum + m * a.lds + i, t[c]);
-      }
+      for (int c = 0; c < C; c++) put8((T*)a.sum + m * a.lds, (c * TPR + at) * 8, n, t[c]);
     }
     unsigned top = 0;
 #pragma unroll
@@ -907,7 +1043,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args 
       for (int e = 0; e < 8; e++) {
         t[c][e] = t[c][e] * r1 * r2 * g[c][e];
         // (past the end of the row t is 0, but 0 times an infinite factor would be NaN)
-        if (OUT == CRNN_E4M3) top = max(top, (c * TPR + at) * 8 < n ? abs_bits(t[c][e]) : 0u);
+        if (OUT == CRNN_E4M3) top = max(top, (c * TPR + at) * 8 + e < n ? abs_bits(t[c][e]) : 0u);
       }
     float ic = 1.f;
     if (OUT == CRNN_E4M3) {
@@ -917,25 +1053,20 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args 
     }
 #pragma unroll
     for (int c = 0; c < C; c++) {
-      const int i = (c * TPR + at) * 8;
       if (OUT == CRNN_E4M3) {
 #pragma unroll
         for (int e = 0; e < 8; e++) t[c][e] *= ic;
       }
-      if (i < n) store8((TO*)a.y + m * a.ldy + i, t[c]);
+      put8((TO*)a.y + m * a.ldy, (c * TPR + at) * 8, n, t[c]);
     }
   }
 }
 
 template <int IN, int OUT>
 static void rms_norm_of(const crnn_rms_norm_args& a, hipStream_t s) {
-  // whole 16-byte chunks in every row (8 bytes where the output is 8 bits)
-  const int64_t ei = IN == CRNN_FP32 ? 4 : 2, eo = OUT == CRNN_E4M3 ? 1 : ei, wo = OUT == CRNN_E4M3 ? 8 : 16;
-  auto fits = [](const void* p, int64_t ld, int64_t e, int64_t w) { return !p || (((uintptr_t)p | (uintptr_t)(ld * e)) & (uintptr_t)(w - 1)) == 0; };
-  const bool wide = a.n % 8 == 0 && a.n <= 8192 && fits(a.x, a.ldx, ei, 16) && fits(a.residual, a.ldr, ei, 16) && fits(a.sum, a.lds, ei, 16) && fits(a.y, a.ldy, eo, wo);
   // at most 8 workgroups a CU at a time: more rows are taken in turn, with the gain at hand
   auto grid = [&](int rows) { return dim3((unsigned)((a.m + rows - 1) / rows < 2048 ? (a.m + rows - 1) / rows : 2048)); };
-  if (!wide) hipLaunchKernelGGL((rms_norm_any_kernel<IN, OUT>), grid_for(a.m), dim3(256), 0, s, a);
+  if (a.n > 8192) hipLaunchKernelGGL((rms_norm_any_kernel<IN, OUT>), grid_for(a.m), dim3(256), 0, s, a);
   else if (a.n <= 512) hipLaunchKernelGGL((rms_norm_kernel<IN, OUT, 64, 1>), grid(4), dim3(256), 0, s, a);
   else if (a.n <= 1024) hipLaunchKernelGGL((rms_norm_kernel<IN, OUT, 64, 2>), grid(4), dim3(256), 0, s, a);
   else if (a.n <= 2048) hipLaunchKernelGGL((rms_norm_kernel<IN, OUT, 64, 4>), grid(4), dim3(256), 0, s, a);

@@ -136,6 +136,33 @@ def test_linear_activations_of_nan_and_infinity(crnn, act, dt):
         torch.testing.assert_close(got.cpu(), want.to(torch.bfloat16).expand(m, 64), rtol=2.0 ** -7, atol=0, equal_nan=True, msg=lambda t: "%d x %d: %s" % (m, k, t))
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "e4m3"])
+@pytest.mark.parametrize("m, k, n", [(1, 4097, 33), (1, 63, 5003), (2, 515, 700), (4, 1031, 4099), (6, 3, 70), (13, 4093, 97), (100, 65, 2100), (4000, 261, 1030), (5000, 3, 2100),
+                                     (2100, 1, 2050), (1500, 2047, 1500)])
+def test_linear_rows_at_any_alignment(crnn, m, k, n, dt):
+    """Odd lengths, and the same rows cut from wider ones at an odd place: what lies beside them (NaN) is not looked at."""
+    x, w, sc = linear_inputs(m, k, n, dt, m + k)
+    bias, res = randn(gen(1), n), randn(gen(2), m, n)
+    for out in ("fp32", "bf16"):
+        r = res.to(DT[out])
+        got = crnn.linear(x, w, bias=bias, residual=r, act="silu", out_dtype=DT[out], **sc)
+        R.check(got, *R.linear(x, w, bias, r, "silu", out_dtype=DT[out], **sc), what=out)
+        X, W = (torch.full((t.shape[0], k + 7), float("nan"), device="cuda").to(DT[dt]) for t in (x, w))
+        X[:, 3:3 + k], W[:, 3:3 + k] = x, w
+        assert torch.equal(crnn.linear(X[:, 3:3 + k], W[:, 3:3 + k], bias=bias, residual=r, act="silu", out_dtype=DT[out], **sc), got)
+
+
+def test_linear_fp32_infinities_at_any_alignment(crnn):
+    g = gen(12)
+    x, w = randn(g, 700, 259), randn(g, 2060, 259)
+    clean = crnn.linear(x, w)
+    x[17, 3], x[650, 258] = float("inf"), -float("inf")
+    got = crnn.linear(x, w)
+    assert torch.equal(got[17], torch.sign(w[:, 3]) * float("inf")) and torch.equal(got[650], -torch.sign(w[:, 258]) * float("inf"))
+    keep = [i for i in range(700) if i not in (17, 650)]
+    assert torch.equal(got[keep], clean[keep])
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e-10, 1e10, 1e18])
 def test_linear_fp32_over_its_range(crnn, scale):
     g = gen(6)
@@ -190,6 +217,21 @@ def test_rms_norm(crnn, m, n, dt):
     for r in (None, res):
         for out in (None, torch.float8_e4m3fn):
             check_norm(crnn, x, gain, r, 1e-6, out)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("m, n", [(3, 2), (9, 9), (300, 511), (2100, 1023), (41, 2047), (20, 4095), (9, 8191), (5, 8193)])
+def test_rms_norm_rows_at_any_alignment(crnn, m, n, dt):
+    g = gen(n)
+    X, Y = (torch.full((m, n + 5), float("nan"), device="cuda").to(DT[dt]) for _ in range(2))
+    X[:, 1:1 + n], Y[:, 3:3 + n] = randn(g, m, n, dt=dt), randn(g, m, n, dt=dt)
+    x, r, gain = X[:, 1:1 + n], Y[:, 3:3 + n], 1 + 0.1 * randn(g, n)
+    for out in (DT[dt], DT["e4m3"]):
+        got = check_norm(crnn, x, gain, r, 1e-6, out)
+        whole = crnn.rms_norm(x.contiguous(), gain, residual=r.contiguous(), out_dtype=out)
+        bits = lambda t: t.view(torch.uint8) if t.dtype is DT["e4m3"] else t
+        again = crnn.rms_norm(x, gain, residual=r, out_dtype=out)
+        assert torch.equal(bits(again.y), bits(whole.y)) and torch.equal(again.sum, whole.sum)
 
 
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
