@@ -338,24 +338,20 @@ template <typename T, int EPC> struct Chunk {
   typedef int raw __attribute__((ext_vector_type(EPC * sizeof(T) / 4)));
   typedef int raw_at __attribute__((ext_vector_type(EPC * sizeof(T) / 4), aligned(sizeof(T))));
   static __device__ __forceinline__ raw whole(const T* p) { return *(const raw_at*)p; }
-  static __device__ __forceinline__ raw any(const T* row, int64_t k0, int64_t k) {
-    raw v = {};
-    if (k0 >= k) return v;
-    if (k0 + EPC <= k) return whole(row + k0);
-    typedef typename std::conditional<sizeof(raw) == 16, unsigned __int128, unsigned long long>::type bits;
-    if (k >= EPC) return __builtin_bit_cast(raw, __builtin_bit_cast(bits, whole(row + k - EPC)) >> (int)((k0 - (k - EPC)) * sizeof(T) * 8));
-    bits b = 0;
-#pragma unroll
-    for (int e = EPC - 1; e >= 0; e--) {
-      typedef typename std::conditional<sizeof(T) == 4, unsigned, typename std::conditional<sizeof(T) == 2, unsigned short, unsigned char>::type>::type word;
-      b = (b << (sizeof(T) * 8)) | (k0 + e < k ? ((const word*)row)[k0 + e] : 0);
-    }
+  typedef typename std::conditional<sizeof(raw) == 16, unsigned __int128, unsigned long long>::type bits;
+  typedef typename std::conditional<sizeof(T) == 4, unsigned, typename std::conditional<sizeof(T) == 2, unsigned short, unsigned char>::type>::type word;
+  static __device__ __forceinline__ raw cut(const T* row, int64_t k0, int64_t k) {   // (k0 below k)
+    const int64_t at = k0 + EPC <= k ? k0 : k - EPC;
+    if (k >= EPC) return __builtin_bit_cast(raw, __builtin_bit_cast(bits, whole(row + at)) >> (int)((k0 - at) * sizeof(T) * 8));
+    bits b = 0;   // (a row shorter than a chunk)
+#pragma unroll 1
+    for (int e = (int)k - 1; e >= 0; e--) b = (b << (sizeof(T) * 8)) | ((const word*)row)[e];
     return __builtin_bit_cast(raw, b);
   }
   // `row` exists or the chunk is zeros; `inside`: it ends before k, for every lane
   static __device__ __forceinline__ raw get(const T* row, int64_t k0, int64_t k, bool exists, bool inside) {
     raw v = {};
-    if (exists) v = inside ? whole(row + k0) : any(row, k0, k);
+    if (exists && (inside || k0 < k)) v = inside ? whole(row + k0) : cut(row, k0, k);
     return v;
   }
 };
@@ -367,19 +363,21 @@ template <typename T, int EPC> struct Chunk {
 // only 13 bits below the largest of each few products that they add first (measured: 2^8 + 2^-5 in one group is exact,
 // 2^8 + 2^-6 is 2^8; between groups and with the accumulator all 24 bits are kept), too few for results in 32 bits.
 // ---------------------------------------------------------------------------
-template <int IN, int OUT, int MT, int NT, int KG>
-__global__ __launch_bounds__(256 * KG, 2) void linear_loose_kernel(const crnn_linear_args a) {
+template <int IN, int OUT, int MT, int NT, int WN, int KG>
+__global__ __launch_bounds__(128 * WN * KG, 2) void linear_loose_kernel(const crnn_linear_args a) {
   typedef typename TypeOf<IN>::t T;
   constexpr bool F32 = IN == CRNN_FP32;
   typedef Slice<F32 ? CRNN_E4M3 : CRNN_BF16> S;   // (fp32: 32 bytes a lane)
   constexpr int RB = 128, NKS = RB / S::KB, KE = F32 ? 32 : 64, EPC = KE / 8;   // bytes of a row of a step in LDS, slices, values, of a chunk
-  constexpr int BM = 64 * MT, BN = 64 * NT, STAGE = (BM + BN) * RB, CH = (BM + BN) / 32;   // chunks of a thread and step
-  constexpr int JOIN = (KG - 1) * 4 * MT * NT * 4096;   // bytes of the other groups' sums
+  constexpr int NW = 2 * WN, TH = 64 * NW, BM = 64 * MT, BN = 32 * WN * NT, STAGE = (BM + BN) * RB;
+  constexpr int RPC = TH / 8, LX = BM / RPC, CH = (BM + BN) / RPC;   // rows of all threads' chunks, chunks of a thread and step (of x, all)
+  constexpr int JOIN = (KG - 1) * NW * MT * NT * 4096;   // bytes of the other groups' sums
   __shared__ __attribute__((aligned(1024))) unsigned char smem_all[KG * 2 * STAGE];
-  static_assert(sizeof(smem_all) >= JOIN + 4 * 4096 * NT, "the epilogue's exchange fits");
+  static_assert(BM % RPC == 0, "a thread's chunk is of x or of w");
+  static_assert(sizeof(smem_all) >= JOIN + NW * 4096 * NT, "the epilogue's exchange fits");
   typedef Chunk<T, EPC> C;
-  const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-  const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wm = wave >> 1, wn = wave & 1;
+  const int tid = threadIdx.x % TH, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x / TH), wm = wave / WN, wn = wave % WN;
   unsigned char* smem = smem_all + kg * 2 * STAGE;
   auto swizzle = [](int r) { return (r >> 1) & 7; };
   const int64_t ntm = (a.m + BM - 1) / BM, ntn = (a.n + BN - 1) / BN, total = ntm * ntn, per = (total + 7) / 8;
@@ -389,23 +387,24 @@ __global__ __launch_bounds__(256 * KG, 2) void linear_loose_kernel(const crnn_li
     if (t0 >= total) break;
     const int64_t grp = t0 / (8 * ntn), in = t0 - grp * 8 * ntn, gm = min((int64_t)8, ntm - grp * 8);
     const int64_t m0 = (grp * 8 + in % gm) * BM, n0 = in / gm * BN;
+    // chunk i of this thread: tid & 7 of row tid / 8 + RPC i, of x below LX
+    const T* px = (const T*)a.x + (m0 + (tid >> 3)) * a.ldx;
+    const T* pw = (const T*)a.w + (n0 + (tid >> 3)) * a.ldw;
+    const int left_x = (int)min(a.m - m0 - (tid >> 3), (int64_t)BM), left_w = (int)min(a.n - n0 - (tid >> 3), (int64_t)BN);
     typename C::raw st[CH];
     auto fetch = [&](int64_t step) __attribute__((always_inline)) {
       const int64_t ks = (step * KG + kg) * KE, k0 = ks + (tid & 7) * EPC;
       const bool inside = ks + KE <= a.k;   // (the same for all)
+      int64_t hx = RPC * a.ldx, hw = RPC * a.ldw;
+      asm volatile("" : "+s"(hx), "+s"(hw));   // (else every chunk's address is kept in registers over the loop)
 #pragma unroll
-      for (int i = 0; i < CH; i++) {
-        const int r = (tid >> 3) + 32 * i;   // 32 i below BM: a row of x
-        const bool isx = 32 * i < BM;
-        const int64_t row = isx ? m0 + r : n0 + r - BM;
-        const T* p = isx ? (const T*)a.x + row * a.ldx : (const T*)a.w + row * a.ldw;
-        st[i] = C::get(p, k0, a.k, row < (isx ? a.m : a.n), inside);
-      }
+      for (int i = 0; i < CH; i++)
+        st[i] = i < LX ? C::get(px + i * hx, k0, a.k, RPC * i < left_x, inside) : C::get(pw + (i - LX) * hw, k0, a.k, RPC * (i - LX) < left_w, inside);
     };
     auto put_stage = [&](int stage) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < CH; i++) {
-        const int r = (tid >> 3) + 32 * i;
+        const int r = (tid >> 3) + RPC * i;
         i32x4 v;
         if constexpr (IN == CRNN_E4M3) {
           bf16x8 b;
@@ -480,7 +479,7 @@ __global__ __launch_bounds__(256 * KG, 2) void linear_loose_kernel(const crnn_li
 #pragma unroll
           for (int j = 0; j < MT; j++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) part[((kg - 1) * 4 * MT * NT * 16 + (i * MT + j) * 16 + r) * 64] = acc[i][j][r];
+            for (int r = 0; r < 16; r++) part[((kg - 1) * NW * MT * NT * 16 + (i * MT + j) * 16 + r) * 64] = acc[i][j][r];
       }
       meet();
       if (kg == 0) {
@@ -491,12 +490,14 @@ __global__ __launch_bounds__(256 * KG, 2) void linear_loose_kernel(const crnn_li
 #pragma unroll
             for (int j = 0; j < MT; j++)
 #pragma unroll
-              for (int r = 0; r < 16; r++) acc[i][j][r] += part[(k * 4 * MT * NT * 16 + (i * MT + j) * 16 + r) * 64];
+              for (int r = 0; r < 16; r++) acc[i][j][r] += part[(k * NW * MT * NT * 16 + (i * MT + j) * 16 + r) * 64];
       }
     }
     if (kg == 0) {
       if constexpr (F32) finite_sums<MT, NT>(a, acc, m0 + wm * 32 * MT, n0 + wn * 32 * NT, lane);
-      linear_out<IN, OUT, MT, NT>(a, acc, smem_all + JOIN + wave * 4096 * NT, m0 + wm * 32 * MT, n0 + wn * 32 * NT, lane);
+      int l = lane;
+      asm volatile("" : "+v"(l));   // (else what only the way out needs is kept in registers over the loop)
+      linear_out<IN, OUT, MT, NT>(a, acc, smem_all + JOIN + wave * 4096 * NT, m0 + wm * 32 * MT, n0 + wn * 32 * NT, l);
     }
     meet();   // (the next tile's operands)
   }
@@ -815,13 +816,15 @@ static void linear_tile(const crnn_linear_args& a, hipStream_t s) {
   const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 32 * WN * NT - 1) / (32 * WN * NT));
   hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT, WN, RB, NST, KG>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(128 * WN * KG), 0, s, a);
 }
+static double tile_rounds(const crnn_linear_args& a, int bm, int bn, int at_once) {
+  return (double)(((a.m + bm - 1) / bm * ((a.n + bn - 1) / bn) + at_once - 1) / at_once);
+}
 template <int IN, int OUT>
 static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
   if ((a.m + 63) / 64 * ((a.n + 63) / 64) >= 1 << 22) return false;   // (a launch has fewer than 2^32 threads)
   // Tiles come in rounds of what the 256 CUs hold; a round takes its tile's size (256 x 256: 4), 128 x 128 ones two a CU with
   // less use of what is loaded.  18176 x 512 x 2048: 256 rows 54 us, 192 rows 50, 128 x 128 59; 16384 x 4096 x 4096: 455, 488, 556.
-  auto rounds = [&](int bm, int bn, int at_once) { return (double)(((a.m + bm - 1) / bm * ((a.n + bn - 1) / bn) + at_once - 1) / at_once); };
-  const double c4 = 4.0 * rounds(256, 256, 256), c3 = 3.0 * rounds(192, 256, 256), c2 = 2.4 * rounds(128, 128, 512);
+  const double c4 = 4.0 * tile_rounds(a, 256, 256, 256), c3 = 3.0 * tile_rounds(a, 192, 256, 256), c2 = 2.4 * tile_rounds(a, 128, 128, 512);
   const int64_t small = ((a.m + 127) / 128) * ((a.n + 127) / 128), tiny = ((a.m + 63) / 64) * ((a.n + 31) / 32);
   if constexpr (IN != CRNN_FP32) {
     if (c4 <= c3 && c4 <= c2) return linear_tile<IN, OUT, 4, 2, 4, 128, 2>(a, s), true;
@@ -854,10 +857,10 @@ static void linear_vector(const crnn_linear_args& a, hipStream_t s) {
   else if (a.m == 2) linear_vector<IN, OUT, 2, CHUNKS>(a, s);
   else linear_vector<IN, OUT, 4, CHUNKS>(a, s);
 }
-template <int IN, int OUT, int MT, int KG>
+template <int IN, int OUT, int MT, int NT, int WN, int KG>
 static void linear_loose(const crnn_linear_args& a, hipStream_t s) {
-  const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 64 * MT - 1) / (64 * MT));
-  hipLaunchKernelGGL((linear_loose_kernel<IN, OUT, MT, MT, KG>), dim3((unsigned)(total < (1 << 20) ? (total + 7) / 8 * 8 : 1 << 20)), dim3(256 * KG), 0, s, a);
+  const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 32 * WN * NT - 1) / (32 * WN * NT));
+  hipLaunchKernelGGL((linear_loose_kernel<IN, OUT, MT, NT, WN, KG>), dim3((unsigned)(total < (1 << 20) ? (total + 7) / 8 * 8 : 1 << 20)), dim3(128 * WN * KG), 0, s, a);
 }
 
 template <int IN, int OUT>
@@ -870,9 +873,13 @@ static void linear_of(const crnn_linear_args& a, hipStream_t s) {
     if (chunks && linear_tiles<IN, OUT>(a, s)) return;
   }
   const int64_t small = ((a.m + 127) / 128) * ((a.n + 127) / 128), tiny = ((a.m + 63) / 64) * ((a.n + 63) / 64);
-  if (small >= 256) linear_loose<IN, OUT, 2, 1>(a, s);
-  else if (tiny <= 256) linear_loose<IN, OUT, 1, 2>(a, s);
-  else linear_loose<IN, OUT, 1, 1>(a, s);
+  // (as in linear_tiles; 9000 x 1023 x 1023: 192 x 256 in one round 43 us, 128 x 128 in two 54)
+  if constexpr (IN != CRNN_FP32) {
+    if (3.0 * tile_rounds(a, 192, 256, 256) <= 1.9 * tile_rounds(a, 128, 128, 512)) return linear_loose<IN, OUT, 3, 2, 4, 1>(a, s);
+  }
+  if (small >= 256) linear_loose<IN, OUT, 2, 2, 2, 1>(a, s);
+  else if (tiny <= 256) linear_loose<IN, OUT, 1, 1, 2, 2>(a, s);
+  else linear_loose<IN, OUT, 1, 1, 2, 1>(a, s);
 }
 
 void launch_linear(const crnn_linear_args& a, hipStream_t s) {
