@@ -251,11 +251,15 @@ CRNN_API int crnn_last_kernel_times(crnn_handle* h, int32_t cap, const char** na
 #define CRNN_ACT_NONE 0
 #define CRNN_ACT_RELU 1
 #define CRNN_ACT_LEAKY 2   /* negative slope 0.2, as the network's leakyRelu */
-#define CRNN_ACT_GELU 3    /* x (1 + erf(x / sqrt 2)) / 2 */
+#define CRNN_ACT_GELU 3    /* x (1 + erf(x / sqrt 2)) / 2, to 2^-23 */
 #define CRNN_ACT_SILU 4    /* x / (1 + exp(-x)) */
+/* All of them keep a NaN; of an infinity they give the limit. */
 
 /* y[i,j] = act( x_scale[i] w_scale[j] sum_k x[i,k] w[j,k] + bias[j] ) + residual[i,j],   i < m, j < n
- * Sums are fp32.  fp32 operands are multiplied with fp32 accuracy. */
+ * Sums are fp32.  fp32 operands are multiplied with fp32 accuracy: as three bfloat16 parts each, of which bits below 2^-126 may
+ * be lost.  8-bit products with bf16 results lose what lies 13 bits below the largest of each eight neighbours along k; with
+ * fp32 results they are exact.  Any strides and alignments; x and w are read fastest where k, ldx, ldw and the pointers are whole
+ * 16-byte chunks. */
 typedef struct {
   int64_t m, n, k;           /* m >= 0 (0: nothing to do), n >= 1, k >= 1; each at most 2^31 - 1 */
   const void* x;             /* [m,k] rows ldx apart, any ldx >= 0 (0: every row the same) */
@@ -301,7 +305,8 @@ CRNN_API int crnn_rms_norm(crnn_handle* h, const crnn_rms_norm_args* a, void* st
  *   s[j] = scale * sum_d q[b,t,h,d] k[b,j,g,d],  p = exp(s - max s),  out[b,t,h,:] = sum_j p[j] v[b,j,g,:] / sum_j p[j]
  * over the keys j < lengths[b] with mask[b,j] != 0, g = h / (heads / kv_heads).  A row without any key is 0.  Keys that are
  * left out are never looked at: whatever their k and v hold (infinities, NaN) changes nothing.  Scores, maxima and sums
- * are fp32; bf16 operands have p rounded to bf16 for the second product. */
+ * are fp32; bf16 operands have p rounded to bf16 for the second product.  Any strides and alignments; where q, k and v, their
+ * strides and head_dim are not whole 16-byte chunks a plain kernel answers, several times slower. */
 typedef struct {
   int64_t batch, q_len, kv_len;   /* batch, q_len, kv_len >= 0; kv_len at most 2^31 - 1 */
   int32_t heads, kv_heads;        /* heads a multiple of kv_heads */

@@ -144,14 +144,19 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
 }
 
 // ---------------------------------------------------------------------------
-// linear, rows of whole 16-byte chunks (bf16, and e4m3 with bf16 results): a tile of 64 NT columns x 64 MT rows of y per
-// workgroup of four waves (2 x 2), a step of 64 bytes of k of every row at a time, straight from memory into one of NST LDS
-// stages.  16-byte chunk c of row r sits at chunk c ^ ((r >> 2) & 3): the 16 rows that ds_read_b128 reads at once are then 16
-// different parts of the 256 bytes that LDS serves in a cycle.  w is the first operand, so that a lane holds four neighbouring
-// columns of one row of y (v_mfma_f32_32x32x16_bf16, two slices a step; 8 bits: v_mfma_f32_32x32x64_f8f6f4, one slice).
-// Each slice's operands are read during the slice before.  One barrier a step, in its last slice: by then everybody has read
-// this step's stage, and the loads for NST steps on go into it; what bounds the loop is their way from memory, so the stages
-// take all of LDS.  Steps past the end load zeros, which keeps the count of loads in flight the same to the last step.
+// linear, rows of whole 16-byte chunks (8 bits: with bf16 results): a tile of 64 MT rows x 32 NT WN columns of y per workgroup,
+// 2 x WN waves of 32 MT x 32 NT each.  A step is 128 bytes of k of every row, straight from memory into one of NST LDS stages.
+// 16-byte chunk c of row r sits at c ^ ((r >> 1) & 7): the 16 rows that ds_read_b128 reads at once then lie in
+// different parts of the 256 bytes that LDS serves in a cycle, and SQ_LDS_BANK_CONFLICT stays 0.  w is the first operand,
+// so that a lane holds four neighbouring columns of one row of y (v_mfma_f32_32x32x16_bf16, four slices a step; 8 bits:
+// v_mfma_f32_32x32x64_f8f6f4, two).  Each slice's operands are read during the slice before.  One barrier a step, in its last
+// slice: by then everybody has read this step's stage, and the loads for NST steps on go into it.  Steps past the end load zeros,
+// which keeps the count of loads in flight the same to the last step.  KG groups of waves take steps in turn and add up at the
+// end where tiles are few.
+// Bound by power where k is long (the chip runs at 1.6 to 1.9 GHz then): bf16 8192 x 8192 x 8192 844 us, 1300 TF/s, which is
+// what the library's product takes; 8 bits 18176 x 2048 x 2048 85 us, 1780 TF/s.  Where k is short, by the way in and out, which nothing
+// hides: 18176 x k x 2048 takes 24 us and 30 more for each 512 of k, 14 of the 24 being the rows that leave.  (One workgroup a CU
+// that loads its next tile before it writes the last: 59 us for k = 512, this 56.)
 // ---------------------------------------------------------------------------
 template <int IN> struct Slice;
 template <> struct Slice<CRNN_BF16> {
@@ -185,9 +190,10 @@ template <> struct Slice<CRNN_FP32> {   // one 16-byte chunk a lane: four v_mfma
 };
 
 // fp32 in three bfloat16 parts: x = h + m + l, each the leading 8 bits of what is left (cut, so the parts are exact and their
-// differences too).  Of the nine products the six largest are multiplied (v_mfma_f32_32x32x16_bf16 at 16 times the rate of the
-// f32 instructions); the others are below 2^-24 of the product.  An infinity makes h infinite and m NaN, and values near the
-// largest may overflow on the way: results that are not finite are computed again by linear_tile_kernel on the f32 instructions.
+// differences too; bits of them below 2^-126 may be lost).  Of the nine products the six largest are multiplied
+// (v_mfma_f32_32x32x16_bf16 at 16 times the rate of the f32 instructions); the others are below 2^-24 of the product.  An
+// infinity makes h infinite and m NaN, and values near the largest may overflow on the way: results that are not finite are
+// computed again (finite_sums).  4096 x 4096 x 4096 717 us, 192 TF/s; on the f32 instructions 1057 us, 130 TF/s.
 struct Parts {
   bf16x8 p[3];
 };
@@ -357,9 +363,10 @@ template <typename T, int EPC> struct Chunk {
 };
 
 // ---------------------------------------------------------------------------
-// linear, any strides, alignments and sizes: as linear_tile_kernel with 32 MT x 32 NT a wave, 2 x 2 waves, but operands go to LDS
-// through registers, because loads straight to LDS want whole 16-byte chunks: a step's loads are on their way while the step
-// before is multiplied.  8-bit values become bfloat16 on the way, which holds them exactly: the 8-bit matrix instructions keep
+// linear, any strides, alignments and sizes: tiles as linear_tile_kernel's, but operands go to LDS through registers, because
+// loads straight to LDS want whole 16-byte chunks: a step's loads are on their way while the step before is multiplied.  Bound
+// by what a CU's cache delivers of rows that cross its lines: bf16 18176 x 2047 x 2048 215 us (2048: 145), 18176 x 511 x 2048
+// 68 us (512: 54).  8-bit values become bfloat16 on the way, which holds them exactly: the 8-bit matrix instructions keep
 // only 13 bits below the largest of each few products that they add first (measured: 2^8 + 2^-5 in one group is exact,
 // 2^8 + 2^-6 is 2^8; between groups and with the accumulator all 24 bits are kept), too few for results in 32 bits.
 // ---------------------------------------------------------------------------
@@ -508,18 +515,17 @@ template <int N> __device__ __forceinline__ void wait_loads() {   // all but the
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
-template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST, int KG>
-__global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_tile_kernel(const crnn_linear_args a) {
+template <int IN, int OUT, int MT, int NT, int WN, int NST, int KG>
+__global__ __launch_bounds__(128 * WN * KG, 2) void linear_tile_kernel(const crnn_linear_args a) {
   constexpr bool F32 = IN == CRNN_FP32;
   typedef Slice<F32 ? CRNN_E4M3 : IN> S;   // (fp32: 32 bytes a lane, as 8 bits)
   typedef typename TypeOf<OUT>::t TO;
-  constexpr int ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1, NKS = RB / S::KB, RPL = 1024 / RB;   // slices of a step, rows of a load
+  constexpr int RB = 128, ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1, NKS = RB / S::KB, RPL = 1024 / RB;   // slices of a step, rows of a load
   constexpr int NW = 2 * WN, BM = 64 * MT, BN = 32 * WN * NT, STAGE = (BM + BN) * RB;
   constexpr int LX = BM / (RPL * NW), LT = (BM + BN) / (RPL * NW);   // dma16 instructions of a wave and step: of x, all
   constexpr int JOIN = (KG - 1) * NW * MT * NT * 4096;   // bytes of the other groups' sums
   __shared__ __attribute__((aligned(1024))) unsigned char smem_all[KG * NST * STAGE];
   static_assert(sizeof(smem_all) >= JOIN + NW * 4096 * NT, "the epilogue's exchange fits");
-  if constexpr (MT * NT > 8) CRNN_WHOLE_REGISTER_FILE();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, half = lane >> 5;
   const int kg = __builtin_amdgcn_readfirstlane(tid >> 6) / NW;
   unsigned char* smem = smem_all + kg * NST * STAGE;
@@ -537,7 +543,7 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
   const i32x4 rx = resource((const char*)a.x + m0 * a.ldx * ES), rw = resource((const char*)a.w + n0 * a.ldw * ES);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
   // lane l of load i of this wave: row r = (wave + NW i) RPL + l / (RB / 16), chunk (l mod RB / 16) ^ swizzle(r), the same for all i
-  auto swizzle = [](int r) { return RB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; };
+  auto swizzle = [](int r) { return (r >> 1) & 7; };
   const int lr = lane / (RB / 16);
   const unsigned cb = (unsigned)(((lane & (RB / 16 - 1)) ^ swizzle(wave * RPL + lr)) * 16);
   static_assert(NW * RPL % 16 == 0, "a load's rows start at the same place of the swizzle");
@@ -572,19 +578,18 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
 #pragma unroll
   for (int t = 0; t < NST; t++)
 #pragma unroll
-    for (int i = 0; i < (NKS > 1 && t == NST - 1 ? LT / 2 : LT); i++) load(t, t, i);
-  wait_loads<(NST - 1) * LT - (NKS > 1 ? LT - LT / 2 : 0)>();
+    for (int i = 0; i < (t == NST - 1 ? LT / 2 : LT); i++) load(t, t, i);
+  wait_loads<(NST - 1) * LT - (LT - LT / 2)>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int f = 0; f < MT + NT; f++) read(0, 0, 0, f);
   int st = 0;
-  // (NKS 1: two steps a turn, so that the operand sets take turns without copies)
 #pragma unroll 1
-  for (int t = 0; t < nk; t += NKS == 1 ? 2 : 1) {
+  for (int t = 0; t < nk; t++) {
 #pragma unroll
-    for (int u = 0; u < (NKS == 1 ? 2 : NKS); u++) {
-      const int set = F32 ? 0 : u & 1, last = NKS == 1 || u == NKS - 1, step = t + (NKS == 1 ? u : 0);
+    for (int u = 0; u < NKS; u++) {
+      const int set = F32 ? 0 : u & 1, last = u == NKS - 1;
       const int nxt = last ? (st + 1 == NST ? 0 : st + 1) : st;
       Parts px[F32 ? MT : 1], pw[F32 ? NT : 1];
       if constexpr (F32) {
@@ -612,11 +617,11 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
         for (int f = q * RPQ; f < (q + 1) * RPQ && f < MT + NT; f++) read(F32 ? 0 : set ^ 1, nxt, last ? 0 : u + 1, f);
         // loads for NST steps on into the stage that the last barrier freed, evenly over the two slices behind it: a burst of
         // them holds the wave up (each takes the address unit, which four waves share, 16 cycles)
-        constexpr int SLOTS = NKS > 1 ? 2 * MT * NT : MT * NT;
+        constexpr int SLOTS = 2 * MT * NT;
         const int p = last ? q : MT * NT + q;
-        if (last || (NKS > 1 && u == 0)) {
+        if (last || u == 0) {
 #pragma unroll
-          for (int l = p * LT / SLOTS; l < (p + 1) * LT / SLOTS; l++) load((last ? step : step - 1) + NST, last ? st : st == 0 ? NST - 1 : st - 1, l);
+          for (int l = p * LT / SLOTS; l < (p + 1) * LT / SLOTS; l++) load((last ? t : t - 1) + NST, last ? st : st == 0 ? NST - 1 : st - 1, l);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -655,11 +660,11 @@ __global__ __launch_bounds__(128 * WN * KG, MT * NT > 8 ? 1 : 2) void linear_til
 }
 
 // ---------------------------------------------------------------------------
-// linear, few rows (at most 32; called for 16) of whole 16-byte chunks: 32 columns of y per workgroup, whose KW waves take 128 bytes of k of
-// every row of w in turn and add up through LDS in a fixed order.  Bound by reading w, or by the way of the first bytes: no
-// LDS on the way in, every lane loads its operands as they lie (the products may be added in any order, so a lane's half of a
-// block is 64 neighbouring bytes), the next block's while this one is multiplied.  x is the first operand: lanes hold
-// neighbouring columns.
+// linear, five to sixteen rows of whole 16-byte chunks: 32 columns of y per workgroup, whose KW waves take 128 bytes of k of every
+// row of w in turn and add up through LDS in a fixed order.  No LDS on the way in, every lane loads its operands as they lie
+// (the products may be added in any order, so a lane's half of a block is 64 neighbouring bytes), the next block's while this
+// one is multiplied.  x is the first operand: lanes hold neighbouring columns.  Bound by reading w, and where n gives few
+// workgroups by what one CU reads: bf16 16 x 512 x 5530 4.6 us, 16 x 8192 x 8192 40 us (3.4 TB/s), 12 x 8192 x 512 25 us.
 // ---------------------------------------------------------------------------
 template <int IN, int OUT, int KW>
 __global__ __launch_bounds__(64 * KW, 2) void linear_rows_kernel(const crnn_linear_args a) {
@@ -725,8 +730,10 @@ __global__ __launch_bounds__(64 * KW, 2) void linear_rows_kernel(const crnn_line
   }
 }
 
-// One to four rows: a wave per NC columns of y, its lanes side by side along k, 16 bytes of every column and row each; fp32 FMAs.
-// Nothing but the first bytes' way and the reading of w: four loads of each column are on their way at a time.
+// One to four rows: a wave per NC columns of y, its lanes side by side along k, 16 bytes of every column and row each; fp32 FMAs
+// (also for 8-bit values with results in 32 bits, since nothing is lost).  Bound by the way of the first bytes, then by reading
+// w: four loads of each column are on their way at a time.  bf16 1 x 512 x 512 3.2 us, 1 x 8192 x 8192
+// 30 us (4.5 TB/s); rows at odd places (CHUNKS false): 1 x 511 x 512 3.8 us, 3 x 8191 x 8192 39 us.
 template <int IN, int OUT, int M, int NC, bool CHUNKS>
 __global__ __launch_bounds__(256, 2) void linear_vector_kernel(const crnn_linear_args a) {
   typedef typename TypeOf<IN>::t T;
@@ -811,10 +818,10 @@ static bool linear_chunks(const crnn_linear_args& a) {
          (256 * (a.ldx > a.ldw ? a.ldx : a.ldw) + a.k) * es < 0x7FFFF000;
 }
 
-template <int IN, int OUT, int MT, int NT, int WN, int RB, int NST, int KG = 1>
+template <int IN, int OUT, int MT, int NT, int WN, int NST, int KG = 1>
 static void linear_tile(const crnn_linear_args& a, hipStream_t s) {
   const int64_t total = ((a.m + 64 * MT - 1) / (64 * MT)) * ((a.n + 32 * WN * NT - 1) / (32 * WN * NT));
-  hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT, WN, RB, NST, KG>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(128 * WN * KG), 0, s, a);
+  hipLaunchKernelGGL((linear_tile_kernel<IN, OUT, MT, NT, WN, NST, KG>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(128 * WN * KG), 0, s, a);
 }
 static double tile_rounds(const crnn_linear_args& a, int bm, int bn, int at_once) {
   return (double)(((a.m + bm - 1) / bm * ((a.n + bn - 1) / bn) + at_once - 1) / at_once);
@@ -827,13 +834,16 @@ static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
   const double c4 = 4.0 * tile_rounds(a, 256, 256, 256), c3 = 3.0 * tile_rounds(a, 192, 256, 256), c2 = 2.4 * tile_rounds(a, 128, 128, 512);
   const int64_t small = ((a.m + 127) / 128) * ((a.n + 127) / 128), tiny = ((a.m + 63) / 64) * ((a.n + 31) / 32);
   if constexpr (IN != CRNN_FP32) {
-    if (c4 <= c3 && c4 <= c2) return linear_tile<IN, OUT, 4, 2, 4, 128, 2>(a, s), true;
-    if (c3 <= c2) return linear_tile<IN, OUT, 3, 2, 4, 128, 2>(a, s), true;
+    if (c4 <= c3 && c4 <= c2) return linear_tile<IN, OUT, 4, 2, 4, 2>(a, s), true;
+    if (c3 <= c2) return linear_tile<IN, OUT, 3, 2, 4, 2>(a, s), true;
   }
-  if (small >= 256) linear_tile<IN, OUT, 2, 2, 2, 128, 2>(a, s);
+  if (small >= 256) linear_tile<IN, OUT, 2, 2, 2, 2>(a, s);
+  // (fp32: a larger tile halves the work of splitting; two groups of waves over k where it leaves CUs with one workgroup.  8000 x 512 x
+  // 512 33 us, 64 x 64 tiles 39; 4544 x 2048 x 512 77 and 87; below 144 tiles too few CUs have work: 2272 x 512 x 512 25 and 19)
+  else if (IN == CRNN_FP32 && small >= 144) linear_tile<IN, OUT, 2, 2, 2, 2, 2>(a, s);
   // (few small tiles: four groups of waves share k.  64 x 2048 x 2048 9.2 us, without 12.5; 300 x 512 x 5530 20 us, without 11)
-  else if (tiny <= 256) linear_tile<IN, OUT, 1, 1, 1, 128, 3, 4>(a, s);
-  else linear_tile<IN, OUT, 1, 1, 2, 128, 3>(a, s);
+  else if (tiny <= 256) linear_tile<IN, OUT, 1, 1, 1, 3, 4>(a, s);
+  else linear_tile<IN, OUT, 1, 1, 2, 3>(a, s);
   return true;
 }
 
@@ -877,6 +887,7 @@ static void linear_of(const crnn_linear_args& a, hipStream_t s) {
   if constexpr (IN != CRNN_FP32) {
     if (3.0 * tile_rounds(a, 192, 256, 256) <= 1.9 * tile_rounds(a, 128, 128, 512)) return linear_loose<IN, OUT, 3, 2, 4, 1>(a, s);
   }
+  // (few small tiles: two groups of waves share k, as in linear_tiles)
   if (small >= 256) linear_loose<IN, OUT, 2, 2, 2, 1>(a, s);
   else if (tiny <= 256) linear_loose<IN, OUT, 1, 1, 2, 2>(a, s);
   else linear_loose<IN, OUT, 1, 1, 2, 1>(a, s);
@@ -938,8 +949,8 @@ template <int TPR> __device__ __forceinline__ unsigned row_max(unsigned v, unsig
   return max(max(part[0], part[1]), max(part[2], part[3]));
 }
 
-// Any strides and sizes: one workgroup per row, the row read again for each of the passes (sum of squares, with 8-bit outputs
-// the largest |y|, the outputs).  The outputs are written in the last pass by the thread that reads the same element, so they
+// Rows longer than 8192: one workgroup per row, the row read again for each of the passes (sum of squares, with 8-bit outputs
+// the largest |y|, the outputs); bound by those readings, element by element: 18176 x 2049 took 180 us here, below 97.  The outputs are written in the last pass by the thread that reads the same element, so they
 // may be the inputs themselves.
 template <int IN, int OUT>
 __global__ __launch_bounds__(256) void rms_norm_any_kernel(const crnn_rms_norm_args a) {
@@ -986,9 +997,11 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(const crnn_rms_norm_a
   }
 }
 
-// Rows of 16-byte chunks that fit the registers of one wave (TPR 64: four rows a workgroup) or one workgroup (TPR 256): x and
-// the residual are read once, everything else happens in registers.  A thread holds C groups of eight values; the gain stays in
-// registers over the rows that a workgroup takes.  Bound by HBM.
+// Rows that fit the registers of one wave (TPR 64: four rows a workgroup) or one workgroup (TPR 256): x and the residual are
+// read once, everything else happens in registers.  A thread holds C groups of eight values, which it loads and stores whole at
+// whatever alignment rows have, one by one where the row ends; the gain stays in registers over the rows that a workgroup takes.
+// Bound by HBM: 18176 x 2048 bf16 with residual and sum to 8 bits 55 us (4.75 TB/s), 18176 x 8192 to bf16 219 us (5.4 TB/s);
+// 18176 x 2047 to 8 bits 75 us, rows crossing cache lines.
 template <int IN, int OUT, int TPR, int C>
 __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args a) {
   typedef typename TypeOf<IN>::t T;
@@ -1097,7 +1110,9 @@ void launch_rms_norm(const crnn_rms_norm_args& a, hipStream_t s) {
 // tiles of keys: M' = max(M, max s), L' = L e^(M - M') + sum e^(s - M'), O' likewise; keys that are left out have s = -inf and
 // v = 0.  While M is -inf nothing has been added (M' - M' is taken as 0).
 //
-// Any strides, sizes and types: 16 rows per workgroup, tiles of 32 keys in LDS as fp32, scores and sums by fp32 FMAs.
+// Any strides, sizes and types: 16 rows per workgroup, tiles of 32 keys in LDS as fp32, scores and sums by fp32 FMAs.  For rows
+// that are not whole 16-byte chunks.  Bound by its LDS reads, two a FMA: bf16 64 lines x 48 queries over 71 states, head_dim 63
+// 73 us, 64 by attention_tile_kernel 9.3.
 // ---------------------------------------------------------------------------
 template <int TYPE>
 __global__ __launch_bounds__(256, 2) void attention_any_kernel(const crnn_cross_attention_args a) {
@@ -1213,6 +1228,10 @@ struct SplitRow {
 // value by value (its rows r and r + 4 half a row apart).  Keys that are left out are never loaded: their
 // offset lies outside the resource, LDS gets zeros, and their score is -inf.
 // With nsplit > 1 workgroups share the keys of one row block and leave (O, M, L) for attention_join_kernel.
+// Bound by both products and the exponentials between them, which the two waves of a SIMD hardly ever do side by side (matrix
+// instructions are busy 37 % of the time, vector ones 46): bf16 8 x 1024 queries of 16 heads over 4096 keys of 4, head_dim 128 305 us, 900 TF/s (two groups
+// of waves in turn 286, and 14 % more at head_dim 64; 64 rows a wave 313 to 387); head_dim 64 181 us.  fp32 by the rate of its
+// instructions: 2 x 1024 queries, head_dim 128 594 us, 116 of 153 TF/s.  Two tiles of keys in LDS and RW 4 are two workgroups a CU.
 template <int TYPE, int DP, int RW, int KW, int KT>
 __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const crnn_cross_attention_args a, int nsplit) {
   typedef typename TypeOf<TYPE>::t T;
@@ -1452,7 +1471,8 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const c
 // each), so an instruction loads 64 / LPK keys; a wave takes chunks of U such groups, the next chunk's loads on their way while
 // this one is worked on.  Every group of lanes keeps a maximum, a sum and a result over its own keys; they are joined at the
 // end, lanes by exchange, the KW waves through LDS, nsplit workgroups by attention_join_kernel.  Keys that are left out are not
-// loaded.  Bound by reading the keys.
+// loaded.  Bound by reading the keys: bf16 256 lines over ragged 71 states of 8 x 64 10.4 us (37 MB if they were full), two over
+// 18176 20.7 us (74 MB).
 template <int TYPE, int LPK, int U, int R, int KW>
 __global__ __launch_bounds__(64 * KW, 2) void attention_few_kernel(const crnn_cross_attention_args a, int nsplit) {
   typedef typename TypeOf<TYPE>::t T;
@@ -1642,7 +1662,8 @@ __global__ __launch_bounds__(64 * KW, 2) void attention_few_kernel(const crnn_cr
 }
 
 // out = sum_s O_s 2^(M_s - M) / sum_s L_s 2^(M_s - M): a workgroup per row, LP lanes with four values each per split, 256 / LP
-// splits side by side, so that everything is asked for at once; the groups meet in LDS.
+// splits side by side, so that everything is asked for at once; the groups meet in LDS.  Bound by the way of the bytes, twice:
+// 3.9 us for 16 rows of 64 splits (one row a thread, split by split: 17).
 template <int TYPE, int LP>
 __global__ __launch_bounds__(256) void attention_join_kernel(const crnn_cross_attention_args a, int nsplit) {
   typedef typename TypeOf<TYPE>::t T;
@@ -1721,7 +1742,8 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
   int64_t blocks, keys;   // row blocks; keys of a workgroup's step
   if (rows <= 4) {
     p.rw = 0;
-    p.kw = a.kv_len <= 128 && bg >= 1024 ? 1 : 4;   // few keys, many heads: a wave a head, nothing to join
+    // few keys, many heads: a wave a head, nothing to join
+    p.kw = a.kv_len <= 128 && bg >= 1024 ? 1 : 4;
     blocks = bg;
     keys = 32 * p.kw;
   } else {
@@ -1736,7 +1758,9 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
     keys = kt * p.kw;
   }
   const int64_t steps = (a.kv_len + keys - 1) / keys;
-  const int64_t fill = p.rw == 0 ? 1024 : 512;                     // workgroups that fill the chip
+  // workgroups that fill the chip: four a CU without matrix instructions (one query over ragged 18176 states: 512 17.6 us, 1024
+  // 16.6), two with them
+  const int64_t fill = p.rw == 0 ? 1024 : 512;
   int64_t ns = blocks >= fill ? 1 : (fill + blocks - 1) / blocks;
   if (p.rw != 0 && ns > steps / 2) ns = steps / 2;                 // at least two steps each
   if (ns > MAX_SPLIT) ns = MAX_SPLIT;
@@ -1838,7 +1862,8 @@ void launch_cross_attention(const crnn_cross_attention_args& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
-// the recogniser's states for the operators above: 16 bytes per thread, zeros behind a line's end
+// the recogniser's states for the operators above: 16 bytes per thread, zeros behind a line's end.  Bound by HBM: 256 lines
+// of 71 states, fp32, @@COPY@@
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void copy_states_kernel(const f32x4* __restrict__ rec, f32x4* __restrict__ out, int32_t* __restrict__ out_len,
                                                           const int32_t* __restrict__ tlen, int64_t total, int row, int T) {

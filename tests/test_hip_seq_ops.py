@@ -152,6 +152,17 @@ def test_linear_rows_at_any_alignment(crnn, m, k, n, dt):
         assert torch.equal(crnn.linear(X[:, 3:3 + k], W[:, 3:3 + k], bias=bias, residual=r, act="silu", out_dtype=DT[out], **sc), got)
 
 
+@pytest.mark.parametrize("m, k, n", [(4600, 520, 512), (2500, 132, 1150), (8000, 4, 500)])
+def test_linear_fp32_tiles_that_share_k(crnn, m, k, n):
+    x, w, _ = linear_inputs(m, k, n, "fp32", 3)
+    bias, res = randn(gen(1), n), randn(gen(2), m, n)
+    R.check(crnn.linear(x, w, bias=bias, residual=res, act="relu"), *R.linear(x, w, bias, res, "relu"))
+    x[m - 1, 1] = float("inf")
+    got = crnn.linear(x, w)
+    assert torch.equal(got[m - 1], torch.sign(w[:, 1]) * float("inf"))
+    R.check(got[:m - 1], *R.linear(x[:m - 1], w))
+
+
 def test_linear_fp32_infinities_at_any_alignment(crnn):
     g = gen(12)
     x, w = randn(g, 700, 259), randn(g, 2060, 259)
