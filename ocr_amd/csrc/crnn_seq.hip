@@ -838,9 +838,9 @@ static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
     if (c3 <= c2) return linear_tile<IN, OUT, 3, 2, 4, 2>(a, s), true;
   }
   if (small >= 256) linear_tile<IN, OUT, 2, 2, 2, 2>(a, s);
-  // (fp32: a larger tile halves the work of splitting; two groups of waves over k where it leaves CUs with one workgroup.  8000 x 512 x
-  // 512 33 us, 64 x 64 tiles 39; 4544 x 2048 x 512 77 and 87; below 144 tiles too few CUs have work: 2272 x 512 x 512 25 and 19)
-  else if (IN == CRNN_FP32 && small >= 144) linear_tile<IN, OUT, 2, 2, 2, 2, 2>(a, s);
+  // (fp32: a larger tile halves the work of splitting; two groups of waves over k where it leaves CUs with one workgroup.
+  // 8000 x 512 x 512, 252 tiles, 33 us, in 64 x 64 ones 39; 4544 x 512 x 512, 144, 31 and 27, too few CUs have work)
+  else if (IN == CRNN_FP32 && small >= 192) linear_tile<IN, OUT, 2, 2, 2, 2, 2>(a, s);
   // (few small tiles: four groups of waves share k.  64 x 2048 x 2048 9.2 us, without 12.5; 300 x 512 x 5530 20 us, without 11)
   else if (tiny <= 256) linear_tile<IN, OUT, 1, 1, 1, 3, 4>(a, s);
   else linear_tile<IN, OUT, 1, 1, 2, 3>(a, s);
@@ -1000,7 +1000,7 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(const crnn_rms_norm_a
 // Rows that fit the registers of one wave (TPR 64: four rows a workgroup) or one workgroup (TPR 256): x and the residual are
 // read once, everything else happens in registers.  A thread holds C groups of eight values, which it loads and stores whole at
 // whatever alignment rows have, one by one where the row ends; the gain stays in registers over the rows that a workgroup takes.
-// Bound by HBM: 18176 x 2048 bf16 with residual and sum to 8 bits 55 us (4.75 TB/s), 18176 x 8192 to bf16 219 us (5.4 TB/s);
+// Bound by HBM: 18176 x 2048 bf16 with residual and sum to 8 bits 55 to 58 us (4.5 TB/s and more), 18176 x 8192 to bf16 219 us (5.4 TB/s);
 // 18176 x 2047 to 8 bits 75 us, rows crossing cache lines.
 template <int IN, int OUT, int TPR, int C>
 __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args a) {
@@ -1863,7 +1863,7 @@ void launch_cross_attention(const crnn_cross_attention_args& a, hipStream_t s) {
 
 // ---------------------------------------------------------------------------
 // the recogniser's states for the operators above: 16 bytes per thread, zeros behind a line's end.  Bound by HBM: 256 lines
-// of 71 states, fp32, @@COPY@@
+// of 280 pixels, fp32, 12.5 us (72 MB)
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void copy_states_kernel(const f32x4* __restrict__ rec, f32x4* __restrict__ out, int32_t* __restrict__ out_len,
                                                           const int32_t* __restrict__ tlen, int64_t total, int row, int T) {

@@ -152,7 +152,7 @@ def test_linear_rows_at_any_alignment(crnn, m, k, n, dt):
         assert torch.equal(crnn.linear(X[:, 3:3 + k], W[:, 3:3 + k], bias=bias, residual=r, act="silu", out_dtype=DT[out], **sc), got)
 
 
-@pytest.mark.parametrize("m, k, n", [(4600, 520, 512), (2500, 132, 1150), (8000, 4, 500)])
+@pytest.mark.parametrize("m, k, n", [(4600, 520, 512), (2500, 132, 1150), (8000, 4, 500), (6200, 520, 512), (2000, 76, 1700)])
 def test_linear_fp32_tiles_that_share_k(crnn, m, k, n):
     x, w, _ = linear_inputs(m, k, n, "fp32", 3)
     bias, res = randn(gen(1), n), randn(gen(2), m, n)
