@@ -49,7 +49,20 @@ class SequenceOps(object):
 
     def _tensors(self, what, names, tensors):
         """Device, gradient and last dimension of every tensor; the stream to run on."""
-        grad = _t.is_grad_enabled()
+        grad, dev = _t.is_grad_enabled(), self.device
+        for t in tensors:
+            if t is not None:
+                try:
+                    if t.get_device() == dev and t.stride(-1) == 1 and not (grad and t.requires_grad):
+                        continue
+                except (AttributeError, IndexError, TypeError):
+                    pass
+                self._refuse(what, names, tensors, grad)
+                break
+        return _stream(dev)
+
+    def _refuse(self, what, names, tensors, grad):
+        """The check in full, for a call that did not pass at first sight (a last dimension of one may have any stride)."""
         for name, t in zip(names, tensors):
             if t is None:
                 continue
@@ -63,17 +76,16 @@ class SequenceOps(object):
                 raise ValueError("%s: %s requires a gradient; these operators are for inference (torch.no_grad())" % (what, name))
             if t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
                 raise ValueError("%s: the last dimension of %s is not contiguous" % (what, name))
-        return _stream(self.device)
 
     @staticmethod
     def _rows(what, name, t, n):
         """(rows, row stride) of a tensor [..., n] whose rows are evenly spaced."""
         shape = t.shape
-        if len(shape) < 1 or shape[-1] != n:
-            raise ValueError("%s: %s has shape %s, its last dimension should be %d" % (what, name, tuple(shape), n))
-        if len(shape) == 2:
+        if len(shape) == 2 and shape[1] == n:
             m = shape[0]
             return (m, t.stride(0)) if m > 1 else (m, n)
+        if len(shape) < 1 or shape[-1] != n:
+            raise ValueError("%s: %s has shape %s, its last dimension should be %d" % (what, name, tuple(shape), n))
         if 0 in shape[:-1]:
             return 0, n
         m, ld, at = 1, None, None
@@ -114,7 +126,7 @@ class SequenceOps(object):
             raise ValueError("linear: unknown activation %r" % (act,))
         n, k = w.shape
         m, ldx = self._rows("linear", "x", x, k)
-        shape = x.shape[:-1] + (n,)
+        shape = (m, n) if x.dim() == 2 else x.shape[:-1] + (n,)
         if out_dtype is None:
             out_dtype = out.dtype if out is not None else _f32 if dt is _f32 else _bf16
         if out_dtype is not _f32 and out_dtype is not _bf16:
@@ -126,7 +138,7 @@ class SequenceOps(object):
         if x_scale is not None and (x_scale.dtype is not _f32 or x_scale.numel() != m or not x_scale.is_contiguous()):
             raise ValueError("linear: x_scale has to be contiguous float32, one per row of x")
         if out is None:
-            out = torch.empty(shape, dtype=out_dtype, device=x.device)
+            out = x.new_empty(shape) if out_dtype is dt else x.new_empty(shape, dtype=out_dtype)
             ldy = n
         else:
             self._like("linear", "out", out, shape, out_dtype)
@@ -163,18 +175,18 @@ class SequenceOps(object):
             raise ValueError("rms_norm: out_dtype has to be x's or float8_e4m3fn, got %s" % (out_dtype,))
         m, ldx = self._rows("rms_norm", "x", x, n)
         if out is None:
-            y, ldy = torch.empty(shape, dtype=out_dtype, device=x.device), n
+            y, ldy = x.new_empty(shape) if out_dtype is dt else x.new_empty(shape, dtype=out_dtype), n
         else:
             self._like("rms_norm", "out", out, shape, out_dtype)
             y, ldy = out, self._rows("rms_norm", "out", out, n)[1]
-        scale = torch.empty(shape[:-1], dtype=_f32, device=x.device) if out_dtype is _e4m3 else None
+        scale = x.new_empty(shape[:-1], dtype=_f32) if out_dtype is _e4m3 else None
         ldr = lds = 0
         total = None
         if residual is not None:
             self._like("rms_norm", "residual", residual, shape, dt)
             ldr = self._rows("rms_norm", "residual", residual, n)[1]
             if sum_out is None:
-                total, lds = torch.empty(shape, dtype=dt, device=x.device), n
+                total, lds = x.new_empty(shape), n
             else:
                 self._like("rms_norm", "sum_out", sum_out, shape, dt)
                 total, lds = sum_out, self._rows("rms_norm", "sum_out", sum_out, n)[1]
@@ -208,7 +220,7 @@ class SequenceOps(object):
         if mask is not None and ((mask.dtype is not torch.bool and mask.dtype is not torch.uint8) or mask.shape != (b, s)):
             raise ValueError("cross_attention: mask has to be bool or uint8 [%d, %d], got %s %s" % (b, s, mask.dtype, tuple(mask.shape)))
         if out is None:
-            out = torch.empty(qs, dtype=dt, device=q.device)
+            out = q.new_empty(qs)
         else:
             self._like("cross_attention", "out", out, qs, dt)
         q1, q2, q3, _ = q.stride()
@@ -222,7 +234,7 @@ class SequenceOps(object):
         need = self._lib.crnn_cross_attention_workspace(self._h, a)
         if need:
             _capi.check(self._h, need)
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device)   # stream-ordered, as all tensors: its memory is free again behind this call
+            ws = q.new_empty(need, dtype=torch.uint8)   # stream-ordered, as all tensors: its memory is free again behind this call
             a = _CROSS_ATTENTION.pack(*args, ws.data_ptr(), need, scale, 0)
         rc = self._lib.crnn_cross_attention(self._h, a, stream)
         if rc:
