@@ -440,6 +440,63 @@ def test_cross_attention_offsets_beyond_32_bits(crnn):
 
 
 # ------------------------------------------------------------------------------------------------------- together
+@pytest.mark.parametrize("k", [4096, 4095])
+def test_rows_beyond_32_bits(crnn, k):
+    """More than 2^31 values in x: aligned rows and rows at any place, linear and rms_norm, at both ends."""
+    g, m, n = gen(5), 530000, 40
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    ends = [0, 1, 2, m // 2, m - 3, m - 2, m - 1]
+    x[ends] = randn(g, len(ends), k, dt="bf16")
+    w, bias, gain = randn(g, n, k, dt="bf16"), randn(g, n), 1 + 0.1 * randn(g, k)
+    y = crnn.linear(x, w, bias=bias)
+    R.check(y[ends], *R.linear(x[ends], w, bias, out_dtype=torch.bfloat16))
+    R.check(y[5:9], *R.linear(x[5:9], w, bias, out_dtype=torch.bfloat16))
+    want = x[ends]
+    norm = crnn.rms_norm(x, gain, out=x)
+    assert norm.y is x
+    t, y, rel = R.rms_norm(want, gain)
+    R.check(x[ends], y, 1.01 * rel * y.abs() + R.ROUND[torch.bfloat16] * y.abs() + R.TINY)
+    assert (x[5:9] == 0).all()
+    del x, norm
+    wide = torch.zeros(40, 1 << 26, dtype=torch.bfloat16, device="cuda")         # few rows, far apart
+    a, out = wide[:, 3:3 + k], wide[:, 1 << 25:(1 << 25) + n]
+    a.copy_(randn(g, 40, k, dt="bf16"))
+    crnn.linear(a, w, bias=bias, out=out)
+    R.check(out, *R.linear(a, w, bias, out_dtype=torch.bfloat16))
+    assert (wide[:, (1 << 25) + n:(1 << 25) + 100] == 0).all() and (wide[:, (1 << 25) - 9:1 << 25] == 0).all()
+
+
+@pytest.mark.parametrize("what", ["linear", "rms_norm", "attention"])
+def test_operators_captured_beside_eager_calls(crnn, what):
+    """Two graphs of one operator, replayed in turn with other eager calls of it between: each has its own outputs and workspace."""
+    g = gen(9)
+    if what == "linear":
+        make = lambda: (randn(g, 70, 515, dt="bf16"), randn(g, 600, 515, dt="bf16"))
+        call = lambda a: crnn.linear(a[0], a[1], act="gelu")
+    elif what == "rms_norm":
+        make = lambda: (randn(g, 70, 515, dt="bf16"), 1 + randn(g, 515))
+        call = lambda a: crnn.rms_norm(a[0], a[1], residual=a[0], out_dtype=torch.float8_e4m3fn).scale
+    else:
+        make = lambda: tuple(randn(g, *t, dt="bf16") for t in ((2, 1, 8, 64), (2, 4000, 8, 64), (2, 4000, 8, 64)))      # splits: a workspace
+        call = lambda a: crnn.cross_attention(*a)
+    sets = [make() for _ in range(3)]
+    want = [call(a).clone() for a in sets]
+    graphs = []
+    for a in sets[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(a)
+        graphs.append((graph, out))
+    for _ in range(4):
+        for (graph, out), w in zip(graphs, want):
+            out.zero_()
+            graph.replay()
+            eager = call(sets[2])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, w) and torch.equal(eager, want[2])
+
+
 def layer_weights(g, dim, heads, d, kvh, dt, q8=False):
     w = {"norm.weight": 1 + 0.1 * randn(g, dim), "q.weight": randn(g, heads * d, dim) / dim ** 0.5, "kv.weight": randn(g, 2 * kvh * d, 512) * 0.2,
          "out.weight": randn(g, dim, heads * d) / (heads * d) ** 0.5, "q.bias": randn(g, heads * d) * 0.1, "out.bias": randn(g, dim) * 0.1}
