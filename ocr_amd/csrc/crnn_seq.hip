@@ -1467,6 +1467,53 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const c
     }
 }
 
+// Lane exchanges without LDS: x of lane ^ F for F 1, 2, 8 (F 4: of the other four of eight lanes, where each four agree), and for 16
+// and 32 both halves' values, in the same order in both.
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+struct Two {
+  float a, b;
+};
+template <int F> __device__ __forceinline__ Two two(float x) {
+  if constexpr (F == 1) return Two{x, dpp<0xB1>(x)};        // quad_perm 1 0 3 2
+  else if constexpr (F == 2) return Two{x, dpp<0x4E>(x)};   // quad_perm 2 3 0 1
+  else if constexpr (F == 8) return Two{x, dpp<0x128>(x)};  // row_ror 8
+  else if constexpr (F == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return Two{__uint_as_float(r[0]), __uint_as_float(r[1])};
+  } else if constexpr (F == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return Two{__uint_as_float(r[0]), __uint_as_float(r[1])};
+  } else {
+    return Two{x, __shfl_xor(x, F)};
+  }
+}
+// Sum over N neighbouring lanes.
+template <int N> __device__ __forceinline__ float group_sum(float x) {
+  x += dpp<0xB1>(x);
+  x += dpp<0x4E>(x);
+  if constexpr (N > 4) x += dpp<0x141>(x);   // row_half_mirror
+  if constexpr (N > 8) x += dpp<0x140>(x);   // row_mirror
+  if constexpr (N > 16) {
+    const Two t = two<16>(x);
+    x = t.a + t.b;
+  }
+  return x;
+}
+// Two groups of lanes' maximum, sum and result become one.
+template <int F, int EPC> __device__ __forceinline__ void join_lanes(float& M, float& L, float (&o)[EPC]) {
+  const Two m = two<F>(M), l = two<F>(L);
+  M = fmaxf(m.a, m.b);
+  const float ms = M == -INFINITY ? 0.f : M, a1 = __builtin_amdgcn_exp2f(m.a - ms), a2 = __builtin_amdgcn_exp2f(m.b - ms);
+  L = l.a * a1 + l.b * a2;
+#pragma unroll
+  for (int i = 0; i < EPC; i++) {
+    const Two t = two<F>(o[i]);
+    o[i] = t.a * a1 + t.b * a2;
+  }
+}
+
 // A few rows (at most four) per key head: no matrix instructions, no LDS on the way in.  LPK lanes share a key (16 bytes of it
 // each), so an instruction loads 64 / LPK keys; a wave takes chunks of U such groups, the next chunk's loads on their way while
 // this one is worked on.  Every group of lanes keeps a maximum, a sum and a result over its own keys; they are joined at the
@@ -1564,9 +1611,7 @@ __global__ __launch_bounds__(64 * KW, 2) void attention_few_kernel(const crnn_cr
         float t = 0.f;
 #pragma unroll
         for (int i = 0; i < EPC; i++) t = fmaf(q[r][i], k[i], t);
-#pragma unroll
-        for (int f = 1; f < LPK; f <<= 1) t += __shfl_xor(t, f);
-        s[r][u] = in ? t : -INFINITY;
+        s[r][u] = in ? group_sum<LPK>(t) : -INFINITY;
       }
     }
     float al[R], Ms[R];
@@ -1610,15 +1655,10 @@ __global__ __launch_bounds__(64 * KW, 2) void attention_few_kernel(const crnn_cr
   }
 #pragma unroll
   for (int r = 0; r < R; r++) {
-#pragma unroll
-    for (int f = LPK; f < 64; f <<= 1) {
-      const float m2 = __shfl_xor(M[r], f), l2 = __shfl_xor(L[r], f), m = fmaxf(M[r], m2), ms = m == -INFINITY ? 0.f : m;
-      const float a1 = __builtin_amdgcn_exp2f(M[r] - ms), a2 = __builtin_amdgcn_exp2f(m2 - ms);
-      L[r] = L[r] * a1 + l2 * a2;
-#pragma unroll
-      for (int i = 0; i < EPC; i++) o[r][i] = o[r][i] * a1 + __shfl_xor(o[r][i], f) * a2;
-      M[r] = m;
-    }
+    if constexpr (LPK <= 4) join_lanes<4>(M[r], L[r], o[r]);
+    if constexpr (LPK <= 8) join_lanes<8>(M[r], L[r], o[r]);
+    if constexpr (LPK <= 16) join_lanes<16>(M[r], L[r], o[r]);
+    join_lanes<32>(M[r], L[r], o[r]);
   }
   if constexpr (KW > 1) {
     if (grp == 0) {
