@@ -32,10 +32,43 @@ template <> struct TypeOf<CRNN_E4M3> { typedef e4m3 t; };
 // FIRST operand's index
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+// Lane exchanges without LDS: x of lane ^ F for F 1, 2, 8 (F 4: of the other four of eight lanes, where each four agree), and for 16
+// and 32 both halves' values, in the same order in both.
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+struct Two {
+  float a, b;
+};
+template <int F> __device__ __forceinline__ Two two(float x) {
+  if constexpr (F == 1) return Two{x, dpp<0xB1>(x)};        // quad_perm 1 0 3 2
+  else if constexpr (F == 2) return Two{x, dpp<0x4E>(x)};   // quad_perm 2 3 0 1
+  else if constexpr (F == 8) return Two{x, dpp<0x128>(x)};  // row_ror 8
+  else if constexpr (F == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return Two{__uint_as_float(r[0]), __uint_as_float(r[1])};
+  } else if constexpr (F == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return Two{__uint_as_float(r[0]), __uint_as_float(r[1])};
+  } else {
+    return Two{x, __shfl_xor(x, F)};
+  }
+}
+// Sum over N neighbouring lanes.
+template <int N> __device__ __forceinline__ float group_sum(float x) {
+  x += dpp<0xB1>(x);
+  x += dpp<0x4E>(x);
+  if constexpr (N > 4) x += dpp<0x141>(x);   // row_half_mirror
+  if constexpr (N > 8) x += dpp<0x140>(x);   // row_mirror
+  if constexpr (N > 16) {
+    const Two t = two<16>(x);
+    x = t.a + t.b;
+  }
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  const Two t = two<32>(group_sum<32>(x));
+  return t.a + t.b;
 }
 
 // x Phi(x) = max(x, 0) - |x| Phi(-|x|), and Phi(-y) = erfc(y / sqrt 2) / 2 by Abramowitz & Stegun 7.1.26: (a1 t + ... + a5 t^5)
@@ -1360,8 +1393,8 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const c
       for (int kb = 0; kb < KT / 32; kb++)
 #pragma unroll
         for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[kb][r]);
-      mt = fmaxf(mt, __shfl_xor(mt, 32));
-      const float Mn = fmaxf(M, mt), Ms = Mn == -INFINITY ? 0.f : Mn * sc;
+      const Two both = two<32>(mt);
+      const float Mn = fmaxf(M, fmaxf(both.a, both.b)), Ms = Mn == -INFINITY ? 0.f : Mn * sc;
       if (__any(Mn > M)) {   // (wave-uniform: most tiles after the first few raise no row's maximum)
         const float al = __builtin_amdgcn_exp2f(M * sc - Ms);
         L *= al;
@@ -1467,40 +1500,6 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const c
     }
 }
 
-// Lane exchanges without LDS: x of lane ^ F for F 1, 2, 8 (F 4: of the other four of eight lanes, where each four agree), and for 16
-// and 32 both halves' values, in the same order in both.
-template <int CTRL> __device__ __forceinline__ float dpp(float x) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
-}
-struct Two {
-  float a, b;
-};
-template <int F> __device__ __forceinline__ Two two(float x) {
-  if constexpr (F == 1) return Two{x, dpp<0xB1>(x)};        // quad_perm 1 0 3 2
-  else if constexpr (F == 2) return Two{x, dpp<0x4E>(x)};   // quad_perm 2 3 0 1
-  else if constexpr (F == 8) return Two{x, dpp<0x128>(x)};  // row_ror 8
-  else if constexpr (F == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return Two{__uint_as_float(r[0]), __uint_as_float(r[1])};
-  } else if constexpr (F == 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return Two{__uint_as_float(r[0]), __uint_as_float(r[1])};
-  } else {
-    return Two{x, __shfl_xor(x, F)};
-  }
-}
-// Sum over N neighbouring lanes.
-template <int N> __device__ __forceinline__ float group_sum(float x) {
-  x += dpp<0xB1>(x);
-  x += dpp<0x4E>(x);
-  if constexpr (N > 4) x += dpp<0x141>(x);   // row_half_mirror
-  if constexpr (N > 8) x += dpp<0x140>(x);   // row_mirror
-  if constexpr (N > 16) {
-    const Two t = two<16>(x);
-    x = t.a + t.b;
-  }
-  return x;
-}
 // Two groups of lanes' maximum, sum and result become one.
 template <int F, int EPC> __device__ __forceinline__ void join_lanes(float& M, float& L, float (&o)[EPC]) {
   const Two m = two<F>(M), l = two<F>(L);
