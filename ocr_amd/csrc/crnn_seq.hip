@@ -1240,7 +1240,7 @@ __device__ __forceinline__ int64_t attention_block(unsigned id, int64_t key_head
 }
 
 // Where split s of nsplit leaves row r of all rows (batch, key head, row): D unnormalised values, then (M, L) behind all of them.
-constexpr int MAX_SPLIT = 64;
+constexpr int MAX_SPLIT = 64, JOIN_ROWS = 1024;
 struct SplitRow {
   float *o, *ml;
   __device__ __forceinline__ SplitRow(const crnn_cross_attention_args& a, int nsplit, int s, int64_t r) {
@@ -1394,9 +1394,9 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const c
 #pragma unroll
         for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[kb][r]);
       const Two both = two<32>(mt);
-      const float Mn = fmaxf(M, fmaxf(both.a, both.b)), Ms = Mn == -INFINITY ? 0.f : Mn * sc;
+      const float Mn = fmaxf(M, fmaxf(both.a, both.b)), Mz = Mn == -INFINITY ? 0.f : Mn, Ms = Mz * sc;
       if (__any(Mn > M)) {   // (wave-uniform: most tiles after the first few raise no row's maximum)
-        const float al = __builtin_amdgcn_exp2f(M * sc - Ms);
+        const float al = __builtin_amdgcn_exp2f((M - Mz) * sc);
         L *= al;
 #pragma unroll
         for (int i = 0; i < DP / 32; i++)
@@ -1408,7 +1408,8 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const c
       for (int kb = 0; kb < KT / 32; kb++) {
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], sc, -Ms));
+          // (fp32: the difference first, so that the largest is exactly 1; one instruction more, which bf16 has no use for)
+          s[kb][r] = __builtin_amdgcn_exp2f(TYPE == CRNN_FP32 ? (s[kb][r] - Mz) * sc : fmaf(s[kb][r], sc, -Ms));
           L += s[kb][r];
         }
         if constexpr (TYPE == CRNN_BF16) {
@@ -1760,6 +1761,38 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const crnn_cross_at
   }
 }
 
+// The same for many rows: LP lanes a row, four values each, 256 / LP rows a workgroup, the splits one after the other.
+template <int TYPE, int LP>
+__global__ __launch_bounds__(256) void attention_join_rows_kernel(const crnn_cross_attention_args a, int nsplit) {
+  typedef typename TypeOf<TYPE>::t T;
+  typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  constexpr int RPB = 256 / LP;
+  const int G = a.heads / a.kv_heads, D = a.head_dim, c = threadIdx.x % LP;
+  const int64_t rows = a.q_len * G, all = a.batch * a.kv_heads * rows;
+  if (4 * c >= D) return;
+  for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LP; r < all; r += (int64_t)gridDim.x * RPB) {
+    float M = -INFINITY;
+#pragma unroll 4
+    for (int s = 0; s < nsplit; s++) M = fmaxf(M, SplitRow(a, nsplit, s, r).ml[0]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < nsplit; s++) {
+      const SplitRow w(a, nsplit, s, r);
+      const float e = __builtin_amdgcn_exp2f(w.ml[0] - Ms);
+      const f32x4 o = *(const f32x4*)(w.o + 4 * c);
+      L = fmaf(w.ml[1], e, L);
+#pragma unroll
+      for (int k = 0; k < 4; k++) v[k] = fmaf(o[k], e, v[k]);
+    }
+    const float d = L == 0.f ? 1.f : L;   // (divided, not multiplied: where one key counts its value comes out as it is)
+    const int64_t bg = r / rows, row = r - bg * rows;
+    T* out = (T*)a.out + bg / a.kv_heads * a.out_stride[0] + row / G * a.out_stride[1] + (bg % a.kv_heads * G + row % G) * a.out_stride[2];
+    *(T4*)(out + 4 * c) = T4{(T)(v[0] / d), (T)(v[1] / d), (T)(v[2] / d), (T)(v[3] / d)};
+  }
+}
+
 static bool attention_chunks(const crnn_cross_attention_args& a) {   // (sizes, type and strides only)
   const int c = a.type == CRNN_BF16 ? 8 : 4;
   if (a.head_dim % c != 0 || a.kv_len == 0 || a.kv_len > 0x7FF00000) return false;   // (key numbers a few steps past the end are ints)
@@ -1797,11 +1830,20 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
     keys = kt * p.kw;
   }
   const int64_t steps = (a.kv_len + keys - 1) / keys;
-  // workgroups that fill the chip: four a CU without matrix instructions (one query over ragged 18176 states: 512 17.6 us, 1024
-  // 16.6), two with them
-  const int64_t fill = p.rw == 0 ? 1024 : 512;
-  int64_t ns = blocks >= fill ? 1 : (fill + blocks - 1) / blocks;
-  if (p.rw != 0 && ns > steps / 2) ns = steps / 2;                 // at least two steps each
+  int64_t ns = 1;
+  if (p.rw == 0) {
+    // four workgroups a CU (one query over ragged 18176 states: 512 in all 17.6 us, 1024 16.6)
+    if (blocks < 1024) ns = (1024 + blocks - 1) / blocks;
+  } else if (blocks < 512) {
+    // two a CU at a time, at least two steps each: rounds of a workgroup's steps and two for its way in and out, and three for
+    // the join.  (Splits that just fill the chip, 512 / blocks rounded up, start a round for its last few: fp32 4 x 400 queries of
+    // 8 heads over 3992 keys, head_dim 128, 347 us, this 256; bf16 30 x 20 queries over 500 keys 20.5 and 11.6.)
+    double best = 0.;
+    for (int64_t n = 1; n <= MAX_SPLIT && (n == 1 || n <= steps / 2); n++) {
+      const double cost = (double)((blocks * n + 511) / 512) * (double)((steps + n - 1) / n + 2) + (n > 1 ? 3. : 0.);
+      if (n == 1 || cost < best) best = cost, ns = n;
+    }
+  }
   if (ns > MAX_SPLIT) ns = MAX_SPLIT;
   if (ns > 1) {                                                    // as many as the steps go into evenly
     const int64_t per = (steps + ns - 1) / ns;
@@ -1862,8 +1904,12 @@ static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p,
 }
 
 template <int TYPE, int LP>
-static void attention_join(const crnn_cross_attention_args& a, int nsplit, dim3 g, hipStream_t s) {
-  hipLaunchKernelGGL((attention_join_kernel<TYPE, LP>), g, dim3(256), 0, s, a, nsplit);
+static void attention_join(const crnn_cross_attention_args& a, int nsplit, hipStream_t s) {
+  const int64_t all = a.batch * a.heads * a.q_len;
+  // a workgroup a row hides the way to memory, a row a few lanes wastes none of it: 8 rows of 64 splits 16.1 and 23.2 us with
+  // the attention, 4800 rows of 5 30.7 and 26.9, 24000 of 2 66 and 38
+  if (all <= JOIN_ROWS) hipLaunchKernelGGL((attention_join_kernel<TYPE, LP>), grid_for(all), dim3(256), 0, s, a, nsplit);
+  else hipLaunchKernelGGL((attention_join_rows_kernel<TYPE, LP>), grid_for((all * LP + 255) / 256), dim3(256), 0, s, a, nsplit);
 }
 
 void launch_cross_attention(const crnn_cross_attention_args& a, hipStream_t s) {
@@ -1889,9 +1935,8 @@ void launch_cross_attention(const crnn_cross_attention_args& a, hipStream_t s) {
     if (p.rw == 0) a.type == CRNN_BF16 ? attention_few<CRNN_BF16>(a, p, s) : attention_few<CRNN_FP32>(a, p, s);
     else a.type == CRNN_BF16 ? attention_tile<CRNN_BF16>(a, p, s) : attention_tile<CRNN_FP32>(a, p, s);
     if (p.nsplit > 1) {
-      const dim3 g = grid_for(a.batch * a.heads * a.q_len);
-      if (a.type == CRNN_BF16) a.head_dim <= 64 ? attention_join<CRNN_BF16, 16>(a, p.nsplit, g, s) : attention_join<CRNN_BF16, 32>(a, p.nsplit, g, s);
-      else a.head_dim <= 64 ? attention_join<CRNN_FP32, 16>(a, p.nsplit, g, s) : attention_join<CRNN_FP32, 32>(a, p.nsplit, g, s);
+      if (a.type == CRNN_BF16) a.head_dim <= 64 ? attention_join<CRNN_BF16, 16>(a, p.nsplit, s) : attention_join<CRNN_BF16, 32>(a, p.nsplit, s);
+      else a.head_dim <= 64 ? attention_join<CRNN_FP32, 16>(a, p.nsplit, s) : attention_join<CRNN_FP32, 32>(a, p.nsplit, s);
     }
     return;
   }

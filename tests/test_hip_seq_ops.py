@@ -386,6 +386,25 @@ def test_cross_attention_many_lines(crnn, b, t, s, d, dt):
         R.check(crnn.cross_attention(q[i:i + 1], k[i:i + 1], v[i:i + 1], lengths=lengths[i:i + 1]), *R.attention(q[i:i + 1], k[i:i + 1], v[i:i + 1], lengths[i:i + 1]))
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("b, t, s, heads, kvh, d", [(2, 300, 1500, 4, 2, 64), (1, 700, 2000, 3, 1, 128), (3, 130, 900, 4, 4, 40), (2, 520, 1100, 2, 2, 32), (1, 256, 3000, 4, 1, 8)])
+def test_cross_attention_many_rows_over_splits(crnn, b, t, s, heads, kvh, d, dt):
+    """Rows that several workgroups share, each part of the keys, more of them than are joined one by one; some without a key."""
+    g = gen(b + t)
+    q, k, v = qkv(g, b, t, s, heads, kvh, d, dt)
+    lengths = torch.tensor([s, 0, s // 3][:b], dtype=torch.int32, device="cuda")
+    mask = torch.rand(b, s, generator=g, device="cuda") < 0.7
+    mask[0, : s // 2] = False                                     # whole splits without a key
+    got = crnn.cross_attention(q, k, v, lengths=lengths, mask=mask)
+    R.check(got, *R.attention(q, k, v, lengths, mask))
+    if b > 1:
+        assert (got[1] == 0).all()
+    buf = torch.full((b, t, heads, d + 3), 7.0, dtype=q.dtype, device="cuda")     # results at any place
+    out = buf[..., 1:1 + d]
+    assert crnn.cross_attention(q, k, v, lengths=lengths, mask=mask, out=out) is out
+    assert torch.equal(out, got) and (buf[..., 0] == 7).all() and (buf[..., 1 + d:] == 7).all()
+
+
 @pytest.mark.parametrize("t, s", [(1, 1), (1, 300), (20, 1), (40, 300)])
 def test_cross_attention_strides_of_single_dimensions_do_not_matter(crnn, t, s):
     g = gen(t + s)
