@@ -1262,8 +1262,8 @@ struct SplitRow {
 // offset lies outside the resource, LDS gets zeros, and their score is -inf.
 // With nsplit > 1 workgroups share the keys of one row block and leave (O, M, L) for attention_join_kernel.
 // Bound by both products and the exponentials between them, which the two waves of a SIMD hardly ever do side by side (matrix
-// instructions are busy 37 % of the time, vector ones 46): bf16 8 x 1024 queries of 16 heads over 4096 keys of 4, head_dim 128 305 us, 900 TF/s (two groups
-// of waves in turn 286, and 14 % more at head_dim 64; 64 rows a wave 313 to 387); head_dim 64 181 us.  fp32 by the rate of its
+// instructions are busy 37 % of the time, vector ones 46): bf16 8 x 1024 queries of 16 heads over 4096 keys of 4, head_dim 128 300 us, 915 TF/s (two groups
+// of waves in turn 286, and 14 % more at head_dim 64; 64 rows a wave 313 to 387); head_dim 64 171 us.  fp32 by the rate of its
 // instructions: 2 x 1024 queries, head_dim 128 594 us, 116 of 153 TF/s.  Two tiles of keys in LDS and RW 4 are two workgroups a CU.
 template <int TYPE, int DP, int RW, int KW, int KT>
 __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const crnn_cross_attention_args a, int nsplit) {
@@ -1518,8 +1518,8 @@ template <int F, int EPC> __device__ __forceinline__ void join_lanes(float& M, f
 // each), so an instruction loads 64 / LPK keys; a wave takes chunks of U such groups, the next chunk's loads on their way while
 // this one is worked on.  Every group of lanes keeps a maximum, a sum and a result over its own keys; they are joined at the
 // end, lanes by exchange, the KW waves through LDS, nsplit workgroups by attention_join_kernel.  Keys that are left out are not
-// loaded.  Bound by reading the keys: bf16 256 lines over ragged 71 states of 8 x 64 10.4 us (37 MB if they were full), two over
-// 18176 20.7 us (74 MB).
+// loaded.  Bound by reading the keys: bf16 256 lines over ragged 71 states of 8 x 64 10.0 us (37 MB if they were full), two over
+// 18176 20.7 us (74 MB).  (Sums over a key's lanes by LDS exchanges: 10.4.)
 template <int TYPE, int LPK, int U, int R, int KW>
 __global__ __launch_bounds__(64 * KW, 2) void attention_few_kernel(const crnn_cross_attention_args a, int nsplit) {
   typedef typename TypeOf<TYPE>::t T;
@@ -1817,7 +1817,8 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
     // few keys, many heads: a wave a head, nothing to join
     p.kw = a.kv_len <= 128 && bg >= 1024 ? 1 : 4;
     blocks = bg;
-    keys = 32 * p.kw;
+    const int64_t chunks = a.head_dim / (a.type == CRNN_BF16 ? 8 : 4);
+    keys = 256 / (chunks <= 4 ? 4 : chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32) * p.kw;
   } else {
     p.rw = rows > 64 ? 4 : rows > 32 ? 2 : 1;
     blocks = bg * ((rows + 32 * p.rw - 1) / (32 * p.rw));
@@ -1830,26 +1831,22 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
     keys = kt * p.kw;
   }
   const int64_t steps = (a.kv_len + keys - 1) / keys;
+  // workgroups at a time: what the registers of a SIMD hold, two a CU, without matrix instructions four for one row and less for
+  // more; steps that each has at least
+  const int64_t b16 = a.type == CRNN_BF16, slots = 256 * (p.rw != 0 ? 2 : rows == 1 ? 4 : (rows == 2 ? 4 : 3) - b16), least = p.rw == 0 ? 1 : 2;
   int64_t ns = 1;
-  if (p.rw == 0) {
-    // four workgroups a CU (one query over ragged 18176 states: 512 in all 17.6 us, 1024 16.6)
-    if (blocks < 1024) ns = (1024 + blocks - 1) / blocks;
-  } else if (blocks < 512) {
-    // two a CU at a time, at least two steps each: rounds of a workgroup's steps and two for its way in and out, and three for
-    // the join.  (Splits that just fill the chip, 512 / blocks rounded up, start a round for its last few: fp32 4 x 400 queries of
-    // 8 heads over 3992 keys, head_dim 128, 347 us, this 256; bf16 30 x 20 queries over 500 keys 20.5 and 11.6.)
+  if (blocks < slots) {
+    // rounds of a workgroup's steps and as many again as the least, for its way in and out, and for the join three and one more
+    // for each 24 splits.  (Splits that just fill the chip, slots / blocks rounded up, start a round for their last few: fp32
+    // 4 x 400 queries of 8 heads over 3992 keys, head_dim 128, 347 us, this 256; bf16 30 x 20 queries over 500 keys 20.5 and
+    // 11.6, 1 over 300 of 100 lines 21.4 and 15.9.)
     double best = 0.;
-    for (int64_t n = 1; n <= MAX_SPLIT && (n == 1 || n <= steps / 2); n++) {
-      const double cost = (double)((blocks * n + 511) / 512) * (double)((steps + n - 1) / n + 2) + (n > 1 ? 3. : 0.);
+    for (int64_t n = 1; n <= MAX_SPLIT && (n == 1 || n * least <= steps); n++) {
+      const double cost = (double)((blocks * n + slots - 1) / slots) * (double)((steps + n - 1) / n + least) + (n > 1 ? 3. + (double)n / 24. : 0.);
       if (n == 1 || cost < best) best = cost, ns = n;
     }
   }
-  if (ns > MAX_SPLIT) ns = MAX_SPLIT;
-  if (ns > 1) {                                                    // as many as the steps go into evenly
-    const int64_t per = (steps + ns - 1) / ns;
-    ns = (steps + per - 1) / per;
-  }
-  p.nsplit = (int)(ns < 1 ? 1 : ns);
+  p.nsplit = (int)ns;
   return p;
 }
 int64_t cross_attention_workspace(const crnn_cross_attention_args& a) {
