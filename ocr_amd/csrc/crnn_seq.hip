@@ -187,8 +187,8 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
 // which keeps the count of loads in flight the same to the last step.  KG groups of waves take steps in turn and add up at the
 // end where tiles are few.
 // Bound by power where k is long (the chip runs at 1.6 to 1.9 GHz then): bf16 8192 x 8192 x 8192 844 us, 1300 TF/s, which is
-// what the library's product takes; 8 bits 18176 x 2048 x 2048 85 us, 1780 TF/s.  Where k is short, by the way in and out, which nothing
-// hides: 18176 x k x 2048 takes 24 us and 30 more for each 512 of k, 14 of the 24 being the rows that leave.  (One workgroup a CU
+// what the library's product takes; 8 bits 18176 x 2048 x 2048 85 us, 1780 TF/s.  Where k is short, by the way in and out, which
+// nothing hides: 18176 x k x 2048 takes 24 us and 30 more for each 512 of k, 14 of the 24 being the rows that leave.  (One workgroup a CU
 // that loads its next tile before it writes the last: 59 us for k = 512, this 56.)
 // ---------------------------------------------------------------------------
 template <int IN> struct Slice;
@@ -766,7 +766,7 @@ __global__ __launch_bounds__(64 * KW, 2) void linear_rows_kernel(const crnn_line
 // One to four rows: a wave per NC columns of y, its lanes side by side along k, 16 bytes of every column and row each; fp32 FMAs
 // (also for 8-bit values with results in 32 bits, since nothing is lost).  Bound by the way of the first bytes, then by reading
 // w: four loads of each column are on their way at a time.  bf16 1 x 512 x 512 3.2 us, 1 x 8192 x 8192
-// 30 us (4.5 TB/s); rows at odd places (CHUNKS false): 1 x 511 x 512 3.8 us, 3 x 8191 x 8192 39 us.
+// 27 us (4.9 TB/s); rows at odd places (CHUNKS false): 1 x 511 x 512 3.8 us, 3 x 8191 x 8192 39 us.
 template <int IN, int OUT, int M, int NC, bool CHUNKS>
 __global__ __launch_bounds__(256, 2) void linear_vector_kernel(const crnn_linear_args a) {
   typedef typename TypeOf<IN>::t T;
@@ -884,15 +884,22 @@ template <int IN, int OUT>
 static void linear_rows(const crnn_linear_args& a, hipStream_t s) {
   constexpr int ES = IN == CRNN_FP32 ? 4 : IN == CRNN_BF16 ? 2 : 1;
   const dim3 g((unsigned)((a.n + 31) / 32));
+  // waves over k: 8 x 512 x 2048 4.1 us with four, 4.8 with sixteen; 8 x 8192 x 2048 26 and 24
   if (a.k * ES <= 1024) hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, 4>), g, dim3(256), 0, s, a);
   else if (a.k * ES <= 4096) hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, 8>), g, dim3(512), 0, s, a);
   else hipLaunchKernelGGL((linear_rows_kernel<IN, OUT, 16>), g, dim3(1024), 0, s, a);
 }
 template <int IN, int OUT, int M, bool CHUNKS>
 static void linear_vector(const crnn_linear_args& a, hipStream_t s) {
-  // (a wave for one column while that does not fill the chip four times over)
-  if (a.n <= 4096) hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 1, CHUNKS>), dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 4, CHUNKS>), dim3((unsigned)((a.n + 15) / 16)), dim3(256), 0, s, a);
+  // A wave takes one column; of many columns for several rows it takes four, which read the rows of x once: 4 x 8192 x 8192
+  // 33 us, by one column 41; 4 x 512 x 5530 7.0 and 6.8; 1 x 8192 x 8192 30 and 27.
+  if constexpr (M > 1) {
+    if (a.n >= 8192) {
+      hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 4, CHUNKS>), dim3((unsigned)((a.n + 15) / 16)), dim3(256), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((linear_vector_kernel<IN, OUT, M, 1, CHUNKS>), dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, s, a);
 }
 template <int IN, int OUT, bool CHUNKS>
 static void linear_vector(const crnn_linear_args& a, hipStream_t s) {
@@ -983,8 +990,8 @@ template <int TPR> __device__ __forceinline__ unsigned row_max(unsigned v, unsig
 }
 
 // Rows longer than 8192: one workgroup per row, the row read again for each of the passes (sum of squares, with 8-bit outputs
-// the largest |y|, the outputs); bound by those readings, element by element: 18176 x 2049 took 180 us here, below 97.  The outputs are written in the last pass by the thread that reads the same element, so they
-// may be the inputs themselves.
+// the largest |y|, the outputs); bound by those readings, element by element: 18176 x 2049 took 180 us here, below 97.  The
+// outputs are written in the last pass by the thread that reads the same element, so they may be the inputs themselves.
 template <int IN, int OUT>
 __global__ __launch_bounds__(256) void rms_norm_any_kernel(const crnn_rms_norm_args a) {
   typedef typename TypeOf<IN>::t T;
@@ -1033,8 +1040,8 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(const crnn_rms_norm_a
 // Rows that fit the registers of one wave (TPR 64: four rows a workgroup) or one workgroup (TPR 256): x and the residual are
 // read once, everything else happens in registers.  A thread holds C groups of eight values, which it loads and stores whole at
 // whatever alignment rows have, one by one where the row ends; the gain stays in registers over the rows that a workgroup takes.
-// Bound by HBM: 18176 x 2048 bf16 with residual and sum to 8 bits 55 to 58 us (4.5 TB/s and more), 18176 x 8192 to bf16 219 us (5.4 TB/s);
-// 18176 x 2047 to 8 bits 75 us, rows crossing cache lines.
+// Bound by HBM: 18176 x 2048 bf16 with residual and sum to 8 bits 55 to 58 us (4.5 TB/s and more), 18176 x 8192 to bf16 219 us
+// (5.4 TB/s); 18176 x 2047 to 8 bits 75 us, rows crossing cache lines.
 template <int IN, int OUT, int TPR, int C>
 __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args a) {
   typedef typename TypeOf<IN>::t T;
@@ -1262,9 +1269,9 @@ struct SplitRow {
 // offset lies outside the resource, LDS gets zeros, and their score is -inf.
 // With nsplit > 1 workgroups share the keys of one row block and leave (O, M, L) for attention_join_kernel.
 // Bound by both products and the exponentials between them, which the two waves of a SIMD hardly ever do side by side (matrix
-// instructions are busy 37 % of the time, vector ones 46): bf16 8 x 1024 queries of 16 heads over 4096 keys of 4, head_dim 128 300 us, 915 TF/s (two groups
-// of waves in turn 286, and 14 % more at head_dim 64; 64 rows a wave 313 to 387); head_dim 64 171 us.  fp32 by the rate of its
-// instructions: 2 x 1024 queries, head_dim 128 594 us, 116 of 153 TF/s.  Two tiles of keys in LDS and RW 4 are two workgroups a CU.
+// instructions are busy 38 % of the time, vector ones 46): bf16 8 x 1024 queries of 16 heads over 4096 keys of 4, head_dim 128,
+// 300 us, 915 TF/s (two groups of waves in turn 286, but 188 for 174 at head_dim 64 and 88 for 69 in small batches; 64 rows a wave
+// 313 to 387); head_dim 64 171 us.  fp32 by the rate of its instructions: 2 x 1024 queries, head_dim 128 594 us, 116 of 153 TF/s.
 template <int TYPE, int DP, int RW, int KW, int KT>
 __global__ __launch_bounds__(64 * RW * KW, 2) void attention_tile_kernel(const crnn_cross_attention_args a, int nsplit) {
   typedef typename TypeOf<TYPE>::t T;
@@ -1812,7 +1819,11 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
   const int64_t rows = a.q_len * (a.heads / a.kv_heads), bg = a.batch * a.kv_heads;
   AttnPlan p;
   int64_t blocks, keys;   // row blocks; keys of a workgroup's step
-  if (rows <= 4) {
+  // Few rows without matrix instructions: bf16 one (1 over 300 keys of 100 lines 16.0 us, by tiles 20.4; 3 over 256 lines of 71
+  // 17.4 and 11.6), with large heads, whose tiles leave a CU one workgroup, three (2 over 600 keys, head_dim 128, 36 and 46; 4
+  // over 2000 20.0 and 17.9), fp32, whose matrix instructions are slow, four (4 over 600 keys, head_dim 128, 73 and 120)
+  const bool b16 = a.type == CRNN_BF16;
+  if (rows <= (!b16 ? 4 : a.head_dim > 64 ? 3 : 1)) {
     p.rw = 0;
     // few keys, many heads: a wave a head, nothing to join
     p.kw = a.kv_len <= 128 && bg >= 1024 ? 1 : 4;
@@ -1833,7 +1844,7 @@ static AttnPlan attention_plan(const crnn_cross_attention_args& a) {
   const int64_t steps = (a.kv_len + keys - 1) / keys;
   // workgroups at a time: what the registers of a SIMD hold, two a CU, without matrix instructions four for one row and less for
   // more; steps that each has at least
-  const int64_t b16 = a.type == CRNN_BF16, slots = 256 * (p.rw != 0 ? 2 : rows == 1 ? 4 : (rows == 2 ? 4 : 3) - b16), least = p.rw == 0 ? 1 : 2;
+  const int64_t slots = 256 * (p.rw != 0 ? 2 : rows == 1 ? 4 : (rows == 2 ? 4 : 3) - b16), least = p.rw == 0 ? 1 : 2;
   int64_t ns = 1;
   if (blocks < slots) {
     // rounds of a workgroup's steps and as many again as the least, for its way in and out, and for the join three and one more
@@ -1887,9 +1898,11 @@ static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p,
 template <int TYPE, int LPK>
 static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {
   const int64_t rows = a.q_len * (a.heads / a.kv_heads);
-  if (rows == 1) attention_few<TYPE, LPK, 1>(a, p, s);
-  else if (rows == 2) attention_few<TYPE, LPK, 2>(a, p, s);
-  else attention_few<TYPE, LPK, 4>(a, p, s);
+  if constexpr (TYPE == CRNN_FP32 || LPK > 8) {   // (bf16 up to head_dim 64: one row, attention_plan)
+    if (rows > 2) return attention_few<TYPE, LPK, 4>(a, p, s);
+    if (rows == 2) return attention_few<TYPE, LPK, 2>(a, p, s);
+  }
+  attention_few<TYPE, LPK, 1>(a, p, s);
 }
 template <int TYPE>
 static void attention_few(const crnn_cross_attention_args& a, const AttnPlan& p, hipStream_t s) {

@@ -387,6 +387,17 @@ def test_cross_attention_many_lines(crnn, b, t, s, d, dt):
 
 
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("d", [16, 64, 72, 128])
+@pytest.mark.parametrize("t, heads, kvh", [(1, 2, 2), (2, 2, 2), (1, 2, 1), (3, 2, 2), (1, 6, 2), (4, 1, 1), (2, 2, 1), (5, 2, 2)])
+def test_cross_attention_one_to_five_rows_a_key_head(crnn, t, heads, kvh, d, dt):
+    for b, s in ((3, 50), (2, 700), (3, 1)):
+        g = gen(b + t + s)
+        q, k, v = qkv(g, b, t, s, heads, kvh, d, dt)
+        lengths = torch.tensor([s, s // 2, 1][:b], dtype=torch.int32, device="cuda")
+        R.check(crnn.cross_attention(q, k, v, lengths=lengths), *R.attention(q, k, v, lengths))
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
 @pytest.mark.parametrize("b, t, s, heads, kvh, d", [(2, 300, 1500, 4, 2, 64), (1, 700, 2000, 3, 1, 128), (3, 130, 900, 4, 4, 40), (2, 520, 1100, 2, 2, 32), (1, 256, 3000, 4, 1, 8)])
 def test_cross_attention_many_rows_over_splits(crnn, b, t, s, heads, kvh, d, dt):
     """Rows that several workgroups share, each part of the keys, more of them than are joined one by one; some without a key."""
