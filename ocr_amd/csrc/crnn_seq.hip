@@ -970,6 +970,17 @@ __device__ __forceinline__ float row_scale(unsigned top) {
   const float t = __uint_as_float(top), low = 448.f * 0x1p-126f;   // (a row of zeros: a scale that divides)
   return (t < low ? low : t) / 448.f;
 }
+// y / c, from 1 / c: the product, and what it leaves of y divided likewise, which a fused multiply-add gives exactly.  (The product
+// alone lies up to 1.5 steps off and takes quotients in the middle between two e4m3 values to the wrong one; v_div_* for each value
+// would be ten instructions for these three.)  An infinite c gives 0, or NaN for an infinite y, as the division does.
+struct RowQuotient {
+  float c, ic;
+  __device__ __forceinline__ explicit RowQuotient(float scale) : c(scale < INFINITY ? scale : 0.f), ic(1.f / scale) {}
+  __device__ __forceinline__ float of(float y) const {
+    const float q = y * ic;
+    return copysignf(fmaf(fmaf(-q, c, y), ic, q), y);   // (-0 stays)
+  }
+};
 
 // Sum over the 64 or 256 threads of a row (256: through LDS, between barriers).
 template <int TPR, typename V> __device__ __forceinline__ V row_sum(V v, V* part) {
@@ -1020,17 +1031,17 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(const crnn_rms_norm_a
       }
       row_factors(row_sum<256>(sd, partd), (double)a.n, a.eps, &r1, &r2);
     }
-    float c = 1.f, ic = 1.f;
+    float c = 1.f;
     if (OUT == CRNN_E4M3) {
       unsigned top = 0;
       for (int64_t i = tid; i < a.n; i += 256) top = max(top, abs_bits(value(i) * r1 * r2 * a.gain[i]));
       c = row_scale(row_max<256>(top, partu));
-      ic = 1.f / c;
     }
+    const RowQuotient by(c);
     for (int64_t i = tid; i < a.n; i += 256) {
       const float t = value(i), y = t * r1 * r2 * a.gain[i];
       if (a.sum) ((T*)a.sum)[m * a.lds + i] = (T)t;
-      store1((TO*)a.y + m * a.ldy + i, OUT == CRNN_E4M3 ? y * ic : y);
+      store1((TO*)a.y + m * a.ldy + i, OUT == CRNN_E4M3 ? by.of(y) : y);
     }
     if (OUT == CRNN_E4M3 && tid == 0) a.y_scale[m] = c;
     __syncthreads();   // (part)
@@ -1105,17 +1116,17 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args 
         // (past the end of the row t is 0, but 0 times an infinite factor would be NaN)
         if (OUT == CRNN_E4M3) top = max(top, (c * TPR + at) * 8 + e < n ? abs_bits(t[c][e]) : 0u);
       }
-    float ic = 1.f;
+    float sc = 1.f;
     if (OUT == CRNN_E4M3) {
-      const float sc = row_scale(row_max<TPR>(top, partu));
-      ic = 1.f / sc;
+      sc = row_scale(row_max<TPR>(top, partu));
       if (at == 0) a.y_scale[m] = sc;
     }
+    const RowQuotient by(sc);
 #pragma unroll
     for (int c = 0; c < C; c++) {
       if (OUT == CRNN_E4M3) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) t[c][e] *= ic;
+        for (int e = 0; e < 8; e++) t[c][e] = by.of(t[c][e]);
       }
       put8((TO*)a.y + m * a.ldy, (c * TPR + at) * 8, n, t[c]);
     }
