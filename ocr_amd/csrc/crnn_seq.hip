@@ -222,11 +222,14 @@ template <> struct Slice<CRNN_FP32> {   // one 16-byte chunk a lane: four v_mfma
   }
 };
 
-// fp32 in three bfloat16 parts: x = h + m + l, each the leading 8 bits of what is left (cut, so the parts are exact and their
-// differences too; bits of them below 2^-126 may be lost).  Of the nine products the six largest are multiplied
-// (v_mfma_f32_32x32x16_bf16 at 16 times the rate of the f32 instructions); the others are below 2^-24 of the product.  An
-// infinity makes h infinite and m NaN, and values near the largest may overflow on the way: results that are not finite are
-// computed again (finite_sums).  4096 x 4096 x 4096 717 us, 192 TF/s; on the f32 instructions 1057 us, 130 TF/s.
+// fp32 in three bfloat16 parts: x = h + m + l, each what is left rounded to 8 bits, so that l holds the rest exactly and the parts have
+// either sign (bits of them below 2^-126 may be lost, what a product with subnormal operands taken as 0 loses of a whole
+// operand).  m is at most 2^-8 of x and l 2^-17.  Of the nine products the six largest are multiplied (v_mfma_f32_32x32x16_bf16 at 16
+// times the rate of the f32 instructions); the others come to at most 2^-24 of the product, of either sign.  (Parts that are cut off
+// have x's sign and are twice as large: up to 7.8 2^-24 of a product are missing then, which sums do not average out.  It took
+// 666 us where this takes 722; with v_cvt_pk_bf16_f32 4544 x 512 x 512 34 and 33.)  An infinity makes h infinite and m NaN, a NaN l, and
+// values near the largest may overflow on the way: results that are not finite are computed again (finite_sums).  4096 x 4096 x
+// 4096 722 us, 190 TF/s; on the f32 instructions 1057 us, 130 TF/s.
 struct Parts {
   bf16x8 p[3];
 };
@@ -237,10 +240,14 @@ __device__ __forceinline__ Parts split3(i32x8 raw) {
     i32x4 packed;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      packed[i] = __builtin_amdgcn_perm(raw[2 * i + 1], raw[2 * i], 0x07060302);   // the upper halves of both
+      unsigned up[2];   // (half a step added; l has no bits to round)
 #pragma unroll
-      for (int e = 2 * i; e < 2 * i + 2; e++)
-        if (part < 2) raw[e] = (int)__float_as_uint(__uint_as_float((unsigned)raw[e]) - __uint_as_float((unsigned)raw[e] & 0xFFFF0000u));
+      for (int e = 0; e < 2; e++) {
+        const unsigned r = (unsigned)raw[2 * i + e];
+        up[e] = r + (part < 2 ? 0x8000u : 0u);
+        if (part < 2) raw[2 * i + e] = (int)__float_as_uint(__uint_as_float(r) - __uint_as_float(up[e] & 0xFFFF0000u));
+      }
+      packed[i] = __builtin_amdgcn_perm(up[1], up[0], 0x07060302);   // the upper halves of both
     }
     s.p[part] = __builtin_bit_cast(bf16x8, packed);
   }

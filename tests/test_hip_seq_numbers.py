@@ -59,3 +59,43 @@ def test_rms_norm_8_bit_values_of_infinite_and_tiny_rows(crnn, n):
     c = got.scale.cpu().double()[:, None]
     assert float(c[0]) == 2.0 ** -126 and float(c[1]) < 1.5 * 2.0 ** -126
     assert ((got.y.float().cpu().double() * c - y).abs() <= 2.0 ** -4 * y.abs() + 2.0 ** -10 * c).all()
+
+
+# (m, n): a tile of each shape, and with them each kernel of the products in three parts
+@pytest.mark.parametrize("m, n", [(1, 40), (16, 40), (17, 40), (200, 300), (1500, 700), (3000, 1030), (4100, 1100)])
+@pytest.mark.parametrize("k", [1, 3, 4, 8])
+def test_linear_fp32_products_one_by_one(crnn, m, n, k):
+    """One product per result, operands of full mantissas and one sign.  Rounded to the 8 bits of bfloat16 a value is off by 2^-8 of
+    its power of two, 2^e: so |m| <= 2^-8 2^e, and l, half a step of a number below that, |l| <= 2^-9 2^-8 2^e; what is left
+    after it fits l's 8 bits.  Left out are m l, l m and l l: (2 2^-25 + 2^-34) of the product.  The sum's last addition counts
+    2^-23 of the result (the smaller operand is cut at half a step of the larger one, 2^-24 of it, and the sum rounded, 2^-24), the five
+    before it as much of partial sums that are at most 2 2^-8 of the product."""
+    g = gen(m + k)
+    rel = 2.0 ** -24 + 2.0 ** -34 + 2.0 ** -23 * (1 + 5 * 2.0 ** -7)
+    hard = lambda t: (1 + torch.randint(0, 128, t.shape, generator=g, device="cuda").float() / 128 - 2.0 ** -23).clamp(min=1)
+    for kind in ("hard", "random"):
+        x, w = torch.zeros(m, k, device="cuda"), torch.zeros(n, k, device="cuda")
+        a, b = torch.rand(m, generator=g, device="cuda") + 0.5, torch.rand(n, generator=g, device="cuda") + 0.5
+        if kind == "hard":
+            a, b = hard(a), hard(b)
+            a[::3] = b[::3] = 1 + 2.0 ** -7 - 2.0 ** -23
+        x[:, k // 2], w[:, k // 2] = a, b
+        want = a.double()[:, None] * b.double()
+        off = ((crnn.linear(x, w).double() - want) / want).abs().max()
+        assert off <= rel, (kind, float(off) * 2 ** 24)
+
+
+@pytest.mark.parametrize("m, n", [(17, 40), (1500, 700), (4100, 1100)])
+@pytest.mark.parametrize("k", [3, 8])
+def test_linear_fp32_every_nan_stays(crnn, m, n, k):
+    """NaN of any payload, also those that rounding their bits would carry out of the exponent."""
+    g = gen(m)
+    x, w = randn(g, m, k), randn(g, n, k)
+    clean = crnn.linear(x, w)
+    for bits in (0x7FFFFFFF, -1, 0x7F800001, 0x7FFF7FFF, -0x7FFFFF, 0x7FC00000):
+        xn, wn = x.clone(), w.clone()
+        xn[m - 1, 1], wn[5, k - 1] = (torch.tensor(bits, dtype=torch.int32).view(torch.float32),) * 2
+        got = crnn.linear(xn, wn)
+        assert torch.isnan(got[m - 1]).all() and torch.isnan(got[:, 5]).all(), hex(bits)
+        got[:, 5] = clean[:, 5]
+        assert torch.equal(got[:m - 1], clean[:m - 1])
