@@ -99,3 +99,24 @@ def test_linear_fp32_every_nan_stays(crnn, m, n, k):
         assert torch.isnan(got[m - 1]).all() and torch.isnan(got[:, 5]).all(), hex(bits)
         got[:, 5] = clean[:, 5]
         assert torch.equal(got[:m - 1], clean[:m - 1])
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("n", [8193, 1 << 17, (1 << 20) + 3, 1 << 24, (1 << 27) + 1])
+def test_rms_norm_of_a_long_row(crnn, n, dt):
+    """One value all along, so that sums that lose what they add show it; the bound does not grow with n."""
+    x = torch.full((1, n), 0.3, device="cuda").to(DT[dt])
+    v = float(x[0, 0])
+    x[0, n // 2] = 4 * v
+    gain = torch.ones(n, device="cuda")
+    r = ((v * v * (n - 1) + 16 * v * v) / n + 1e-6) ** -0.5
+    # in 32 bits: the sum, n, their quotient and eps once each, halved by the root, then the root, its inverse and two products
+    rel = (4 / 2 + 4) * 2.0 ** -24 + R.ROUND[DT[dt]]
+    y = crnn.rms_norm(x, gain).y
+    for at, t in ((0, v), (n // 2, 4 * v), (n - 1, v)):
+        assert abs(float(y[0, at]) - t * r) <= rel * t * r, (at, float(y[0, at]), t * r)
+    y[0, n // 2] = y[0, 0]
+    assert (y == y[0, 0]).all()
+    got = crnn.rms_norm(x, gain, out_dtype=DT["e4m3"])
+    # the largest value times 1 / 448, two roundings more
+    assert abs(float(got.scale[0]) * 448 - 4 * v * r) <= ((4 / 2 + 6) * 2.0 ** -24) * 4 * v * r
