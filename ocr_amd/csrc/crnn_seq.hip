@@ -923,7 +923,8 @@ static void linear_loose(const crnn_linear_args& a, hipStream_t s) {
 template <int IN, int OUT>
 static void linear_of(const crnn_linear_args& a, hipStream_t s) {
   const bool chunks = linear_chunks(a);
-  const bool few = a.n < 1 << 26 && a.k < 1 << 28;   // (a launch has fewer than 2^32 threads; places in a row are 32-bit)
+  // (a launch has fewer than 2^32 threads, of which one row takes 64 a column; places in a row are 32-bit)
+  const bool few = a.n <= (1 << 26) - 4 && a.k < 1 << 28;
   if (a.m <= 4 && few) return chunks ? linear_vector<IN, OUT, true>(a, s) : linear_vector<IN, OUT, false>(a, s);
   if constexpr (IN != CRNN_E4M3 || OUT == CRNN_BF16) {
     if (chunks && a.m <= 16 && few) return linear_rows<IN, OUT>(a, s);

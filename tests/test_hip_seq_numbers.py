@@ -120,3 +120,13 @@ def test_rms_norm_of_a_long_row(crnn, n, dt):
     got = crnn.rms_norm(x, gain, out_dtype=DT["e4m3"])
     # the largest value times 1 / 448, two roundings more
     assert abs(float(got.scale[0]) * 448 - 4 * v * r) <= ((4 / 2 + 6) * 2.0 ** -24) * 4 * v * r
+
+
+@pytest.mark.parametrize("k", [1, 8])
+def test_linear_one_row_of_very_many_columns(crnn, k):
+    """On both sides of 2^26 columns, where a wave for each column would take a launch of 2^32 threads."""
+    for n in ((1 << 26) - 4, (1 << 26) - 3, (1 << 26) - 1, (1 << 26) + 5):
+        w = torch.zeros(n, k, dtype=torch.bfloat16, device="cuda")
+        w[:, k // 2] = torch.arange(n, device="cuda") % 251
+        x = torch.ones(1, k, dtype=torch.bfloat16, device="cuda")
+        assert torch.equal(crnn.linear(x, w)[0], w[:, k // 2])
