@@ -198,6 +198,8 @@ class SequenceOps(object):
                 _types[out_dtype], 0), stream)
             if rc:
                 _capi.check(self._h, rc)
+        elif m and scale is not None:
+            scale.fill_(2.0 ** -126)   # rows without values: their largest is 0
         return RmsNorm(y, scale, total)
 
     def cross_attention(self, q, k, v, lengths=None, mask=None, scale=None, out=None):

@@ -185,3 +185,32 @@ def test_the_attention_bound_holds_for_32_bits_and_not_for_a_lost_key():
     z[1, :, :, 16:] = -float("inf")
     with pytest.raises(AssertionError):
         R.check(torch.einsum("bhts,bshd->bthd", torch.softmax(z, 3), v), want, err)
+
+
+def host_face(monkeypatch):
+    """The torch face on host tensors with a library that only remembers its calls: what Python decides before and beside them."""
+    from ocr_amd.crnn import seq_ops
+
+    class Lib(object):
+        def __init__(self):
+            self.calls = []
+
+        def __getattr__(self, name):
+            return lambda *a: self.calls.append(name) or 0
+
+    seq_ops._torch()
+    monkeypatch.setattr(seq_ops, "_stream", lambda device: 0)
+    face = seq_ops.SequenceOps()
+    face.device, face._h, face._lib, face.precision = -1, None, Lib(), "fp32"
+    return face
+
+
+def test_rms_norm_of_rows_without_values_has_its_scale(monkeypatch):
+    """The largest of no values counts as 0: the smallest scale, never what the memory held before."""
+    face = host_face(monkeypatch)
+    monkeypatch.setattr(torch.Tensor, "new_empty", lambda t, shape, dtype=None: torch.full(tuple(shape), 7.0).to(dtype or t.dtype))
+    for shape in ((5, 0), (2, 3, 0)):
+        got = face.rms_norm(torch.zeros(shape), torch.zeros(0), out_dtype=torch.float8_e4m3fn)
+        assert got.y.shape == shape and got.scale.shape == shape[:-1] and (got.scale == 2.0 ** -126).all()
+    assert face.rms_norm(torch.zeros(0, 0), torch.zeros(0), out_dtype=torch.float8_e4m3fn).scale.shape == (0,)
+    assert face._lib.calls == []
