@@ -3,7 +3,8 @@ crnn_cross_attention and crnn_states_device (include/crnn_hip.h), as methods of 
 
 They run on torch's current stream of the handle's device and return without waiting; outputs are new tensors unless
 ``out`` is given.  Tensors have to be on the handle's device, with the last dimension contiguous; anything else about their
-strides is taken as it is.  Inference only: a call that autograd would have to record is refused.
+strides is taken as it is.  Inference only: a call that autograd would have to record is refused, one on tensors with
+forward-mode tangents too.
 """
 import collections
 import struct
@@ -21,6 +22,7 @@ _t = None       # torch, imported by the first call: the recogniser itself does 
 _types = None   # torch dtype -> CRNN_* type
 _f32 = _bf16 = _e4m3 = None
 _stream = None  # device index -> its current stream
+_forward = None  # torch.autograd.forward_ad
 
 # The argument structs of include/crnn_hip.h as they lie in memory: packing a few integers costs a fifth of filling a
 # ctypes.Structure, and a call's host time is what small operators cost.
@@ -30,12 +32,13 @@ _CROSS_ATTENTION = struct.Struct("@3q4i4P12q2Pq" + "Pqfi")
 
 
 def _torch():
-    global _t, _types, _stream, _f32, _bf16, _e4m3
+    global _t, _types, _stream, _forward, _f32, _bf16, _e4m3
     if _t is None:
         import torch
         _f32, _bf16, _e4m3 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
         _types = {_f32: _capi.FP32, _bf16: _capi.BF16, _e4m3: _capi.E4M3}
         _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+        import torch.autograd.forward_ad as _forward
         _t = torch
     return _t
 
@@ -59,7 +62,17 @@ class SequenceOps(object):
                     pass
                 self._refuse(what, names, tensors, grad)
                 break
+        if getattr(_forward, "_current_level", 0) >= 0:   # (within a level of forward-mode derivatives only)
+            self._refuse_tangents(what, names, tensors)
         return _stream(dev)
+
+    @staticmethod
+    def _refuse_tangents(what, names, tensors):
+        if not _t._C._is_fwd_grad_enabled():
+            return
+        for name, t in zip(names, tensors):
+            if t is not None and _forward.unpack_dual(t).tangent is not None:
+                raise ValueError("%s: %s has a forward-mode gradient; these operators are for inference" % (what, name))
 
     def _refuse(self, what, names, tensors, grad):
         """The check in full, for a call that did not pass at first sight (a last dimension of one may have any stride)."""

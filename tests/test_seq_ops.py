@@ -214,3 +214,25 @@ def test_rms_norm_of_rows_without_values_has_its_scale(monkeypatch):
         assert got.y.shape == shape and got.scale.shape == shape[:-1] and (got.scale == 2.0 ** -126).all()
     assert face.rms_norm(torch.zeros(0, 0), torch.zeros(0), out_dtype=torch.float8_e4m3fn).scale.shape == (0,)
     assert face._lib.calls == []
+
+
+def test_forward_mode_tangents_are_refused(monkeypatch):
+    """A tensor with a tangent would come back without one: refused, as what requires a gradient is, unless such derivatives are off."""
+    import torch.autograd.forward_ad as fwd
+    face = host_face(monkeypatch)
+    x, w, q = torch.ones(4, 16), torch.ones(8, 16), torch.ones(2, 3, 4, 8)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for call in (lambda: face.linear(dual(x), w), lambda: face.linear(x, dual(w)), lambda: face.linear(x, w, bias=dual(w[:, 0].contiguous())),
+                     lambda: face.rms_norm(dual(x), x[0]), lambda: face.rms_norm(x, dual(x[0])), lambda: face.rms_norm(x, x[0], residual=dual(x)),
+                     lambda: face.cross_attention(dual(q), q, q), lambda: face.cross_attention(q, q, dual(q))):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="gradient"):      # (no_grad is of reverse mode only)
+                call()
+        assert face._lib.calls == []
+        assert face.linear(x, w).shape == (4, 8)                                 # the level alone is no reason
+        assert face.cross_attention(q, q, q, lengths=torch.ones(2, dtype=torch.int32), mask=torch.ones(2, 3, dtype=torch.bool)).shape == q.shape
+        with torch.inference_mode():
+            assert face.linear(x, w).shape == (4, 8)
+    assert face.linear(x, w).shape == (4, 8) and face._lib.calls == ["crnn_linear", "crnn_cross_attention_workspace", "crnn_cross_attention"] + ["crnn_linear"] * 2
