@@ -21,7 +21,8 @@ class LineAttention(object):
     weights: "norm.weight" float32 [dim]; "q.weight" [heads * d, dim], "kv.weight" [2 * kv_heads * d, 512] (keys before
     values), "out.weight" [dim, heads * d], all float32 or all bfloat16, tensors on the handle's device; optional float32
     biases "q.bias", "kv.bias", "out.bias".  "q.weight" may be float8_e4m3fn with a float32 "q.scale" [heads * d] where the
-    others are bfloat16: the norm then leaves 8-bit rows for it."""
+    others are bfloat16: the norm then leaves 8-bit rows for it.  d is 1 .. 128; heads of whole 16-byte chunks (8 bfloat16, 4
+    float32 values) are several times faster."""
 
     def __init__(self, crnn, weights, heads, kv_heads=None, eps=1e-6):
         import torch
@@ -40,9 +41,16 @@ class LineAttention(object):
         if q.dim() != 2 or heads < 1 or self.kv_heads < 1 or heads % self.kv_heads or q.shape[0] % heads:
             raise ValueError("LineAttention: q.weight %s does not fit %d heads over %d" % (tuple(q.shape), heads, self.kv_heads))
         self.d, self.dim = q.shape[0] // heads, q.shape[1]
-        for name, shape in (("kv.weight", (2 * self.kv_heads * self.d, 512)), ("out.weight", (self.dim, heads * self.d)), ("norm.weight", (self.dim,))):
+        if not 1 <= self.d <= 128:
+            raise ValueError("LineAttention: q.weight %s gives heads of %d, 1 .. 128 are possible" % (tuple(q.shape), self.d))
+        for name, shape in (("kv.weight", (2 * self.kv_heads * self.d, 512)), ("out.weight", (self.dim, heads * self.d))):
             if tuple(self.w[name].shape) != shape:
                 raise ValueError("LineAttention: %s has to be %s, got %s" % (name, shape, tuple(self.w[name].shape)))
+        for name, size in (("norm.weight", self.dim), ("q.bias", heads * self.d), ("q.scale", heads * self.d), ("kv.bias", 2 * self.kv_heads * self.d),
+                           ("out.bias", self.dim)):
+            t = self.w.get(name)
+            if t is not None and (tuple(t.shape) != (size,) or t.dtype is not torch.float32):
+                raise ValueError("LineAttention: %s has to be float32 [%d], got %s %s" % (name, size, t.dtype, tuple(t.shape)))
 
     def memory(self, states, lengths=None):
         """Keys and values of ``states`` [n, T, 512] (``CRNN.line_states``), a memory of its own for each line."""

@@ -236,3 +236,25 @@ def test_forward_mode_tangents_are_refused(monkeypatch):
         with torch.inference_mode():
             assert face.linear(x, w).shape == (4, 8)
     assert face.linear(x, w).shape == (4, 8) and face._lib.calls == ["crnn_linear", "crnn_cross_attention_workspace", "crnn_cross_attention"] + ["crnn_linear"] * 2
+
+
+def test_line_attention_checks_head_size_biases_and_scales():
+    """What no call of the layer could run on is refused where it is made."""
+    from ocr_amd.crnn.attention import LineAttention
+
+    def weights(dim=64, heads=4, d=8, dt=torch.float32, **more):
+        return dict({"norm.weight": torch.ones(dim), "q.weight": torch.zeros(heads * d, dim, dtype=dt), "kv.weight": torch.zeros(2 * heads * d, 512, dtype=dt),
+                     "out.weight": torch.zeros(dim, heads * d, dtype=dt), "q.bias": torch.zeros(heads * d), "kv.bias": torch.zeros(2 * heads * d),
+                     "out.bias": torch.zeros(dim)}, **more)
+    for d in (1, 20, 36, 128):
+        assert LineAttention(None, weights(d=d), heads=4).d == d
+    q8 = dict(weights(dt=torch.bfloat16), **{"q.weight": torch.zeros(32, 64).to(torch.float8_e4m3fn), "q.scale": torch.ones(32)})
+    assert LineAttention(None, q8, heads=4).q8
+    for bad in (weights(d=200), weights(d=129), weights(d=0)):
+        with pytest.raises(ValueError, match="head"):
+            LineAttention(None, bad, heads=4)
+    for w, change in ((weights(), {"q.bias": torch.zeros(31)}), (weights(), {"kv.bias": torch.zeros(32)}), (weights(), {"out.bias": torch.zeros(1, 64)}),
+                      (weights(), {"q.bias": torch.zeros(32).bfloat16()}), (weights(), {"norm.weight": torch.ones(64).bfloat16()}), (q8, {"q.scale": torch.ones(64)}),
+                      (q8, {"q.scale": torch.ones(32).double()})):
+        with pytest.raises(ValueError, match=next(iter(change))):
+            LineAttention(None, dict(w, **change), heads=4)
