@@ -251,7 +251,7 @@ CRNN_API int crnn_last_kernel_times(crnn_handle* h, int32_t cap, const char** na
 #define CRNN_ACT_NONE 0
 #define CRNN_ACT_RELU 1
 #define CRNN_ACT_LEAKY 2   /* negative slope 0.2, as the network's leakyRelu */
-#define CRNN_ACT_GELU 3    /* x (1 + erf(x / sqrt 2)) / 2, to 2^-23 */
+#define CRNN_ACT_GELU 3    /* x (1 + erf(x / sqrt 2)) / 2, off by at most 2^-20 |x| (seen: 2^-21.7): nothing relative where x < 0 */
 #define CRNN_ACT_SILU 4    /* x / (1 + exp(-x)) */
 /* All of them keep a NaN; of an infinity they give the limit. */
 

@@ -130,3 +130,17 @@ def test_linear_one_row_of_very_many_columns(crnn, k):
         w[:, k // 2] = torch.arange(n, device="cuda") % 251
         x = torch.ones(1, k, dtype=torch.bfloat16, device="cuda")
         assert torch.equal(crnn.linear(x, w)[0], w[:, k // 2])
+
+
+@pytest.mark.parametrize("m, k, n", [(1, 1, 60000), (1, 8, 60000), (8, 8, 60000), (40, 8, 2000), (300, 8, 2000), (300, 3, 2000)])
+def test_gelu_over_its_range(crnn, m, k, n):
+    """x (1 + erf(x / sqrt 2)) / 2 at arguments that arrive exactly (the bias of a product of zeros).  Phi(-|x|), which is at most
+    1/2, by a form that is off by 0.75e-7 itself; in units of 2^-24: 1.3 for that, of the evaluation 0.2 for the exponent's
+    argument and 1 for the exponential, 3 roundings of t for up to 1.73 of p, 2 for the polynomial, 0.5 for the product with |x|,
+    and of the result 1."""
+    rel = (1.3 + 0.2 + 1 + 3 * 1.73 + 2 + 0.5 + 1) * 2.0 ** -24
+    z = torch.cat([torch.linspace(-14, 14, n - n // 2), torch.logspace(-30, 1, n // 2 - n // 4), -torch.logspace(-30, 1, n // 4)])
+    w = torch.zeros(n, k, device="cuda")
+    got = crnn.linear(torch.zeros(m, k, device="cuda"), w, bias=z.cuda(), act="gelu").double().cpu()
+    want = R.act64(z.double(), "gelu")
+    assert ((got - want).abs() <= rel * z.double().abs() + R.TINY).all(), float(((got - want).abs() / z.double().abs().clamp(min=1e-30)).max() * 2 ** 24)
