@@ -256,10 +256,11 @@ CRNN_API int crnn_last_kernel_times(crnn_handle* h, int32_t cap, const char** na
 /* All of them keep a NaN; of an infinity they give the limit. */
 
 /* y[i,j] = act( x_scale[i] w_scale[j] sum_k x[i,k] w[j,k] + bias[j] ) + residual[i,j],   i < m, j < n
- * Sums are fp32.  fp32 operands are multiplied with fp32 accuracy: as three bfloat16 parts each, of which bits below 2^-126 may
- * be lost.  8-bit products with bf16 results lose what lies 13 bits below the largest of each eight neighbours along k; with
- * fp32 results they are exact.  Any strides and alignments; x and w are read fastest where k, ldx, ldw and the pointers are whole
- * 16-byte chunks. */
+ * Sums are fp32.  fp32 operands are multiplied to 2^-24 of each product, from 17 rows on (5 where x or w are not whole 16-byte chunks)
+ * as three bfloat16 parts each, of which bits below 2^-126 may be lost; few rows have each product exactly.  8-bit products with
+ * bf16 results lose what lies 13 bits below the largest of each eight neighbours along k (but for up to four rows, and where x or w are
+ * not whole 16-byte chunks); with fp32 results they are exact.  Any strides and alignments; x and w are read fastest where k, ldx,
+ * ldw and the pointers are whole 16-byte chunks. */
 typedef struct {
   int64_t m, n, k;           /* m >= 0 (0: nothing to do), n >= 1, k >= 1; each at most 2^31 - 1 */
   const void* x;             /* [m,k] rows ldx apart, any ldx >= 0 (0: every row the same) */

@@ -125,7 +125,7 @@ class SequenceOps(object):
     def linear(self, x, w, bias=None, residual=None, act="none", x_scale=None, w_scale=None, out_dtype=None, out=None):
         """act(x w^T + bias) + residual: x [..., k], w [n, k], bias float32 [n], residual and the result [..., n].
 
-        x and w are both float32 (multiplied with fp32 accuracy), bfloat16 or float8_e4m3fn; the latter with float32
+        x and w are both float32 (each product to 2^-24), bfloat16 or float8_e4m3fn; the latter with float32
         ``x_scale`` (one per row of x) and ``w_scale`` [n].  act: none, relu, leaky (0.2), gelu, silu.  ``out_dtype``
         float32 or bfloat16: of the result and the residual (default: x's, bfloat16 for float8).  ``out`` may be the
         residual itself."""

@@ -144,3 +144,51 @@ def test_gelu_over_its_range(crnn, m, k, n):
     got = crnn.linear(torch.zeros(m, k, device="cuda"), w, bias=z.cuda(), act="gelu").double().cpu()
     want = R.act64(z.double(), "gelu")
     assert ((got - want).abs() <= rel * z.double().abs() + R.TINY).all(), float(((got - want).abs() / z.double().abs().clamp(min=1e-30)).max() * 2 ** 24)
+
+
+@pytest.mark.parametrize("m, k, n", [(3, 4096, 500), (9, 4096, 500), (48, 8192, 200), (300, 2048, 300), (800, 4096, 1100), (5000, 2048, 1100), (300, 2049, 300)])
+def test_linear_8_bits_one_missing_value_shows(crnn, m, k, n):
+    """Operands of +-1 (and scales of 1): every product and sum is a whole number, exact in each of the kernels."""
+    g = gen(k)
+    x, w = ((torch.rand(r, k, generator=g, device="cuda") < 0.5).float() * 2 - 1 for r in (m, n))
+    want = (x @ w.t()).round()
+    got = crnn.linear(x.to(DT["e4m3"]), w.to(DT["e4m3"]))
+    assert torch.equal(got, want.to(torch.bfloat16))
+    small = want.abs() <= 256                                            # (whole numbers that bfloat16 holds)
+    assert small.float().mean() > 0.9 and torch.equal(got[small].float(), want[small])
+
+
+@pytest.mark.parametrize("m, k, n", [(9, 4096, 500), (48, 8192, 200), (300, 2048, 300), (800, 4096, 1100), (5000, 2048, 1100), (300, 2049, 300)])
+def test_linear_8_bits_error_of_many_results(crnn, m, k, n):
+    """Root mean square and mean of the error over all results.  A product loses less than 2^-13 of the largest of its eight, g,
+    here taken as spread evenly over that: 2^-13 g / sqrt 3 a product, of any sign, sqrt(k) of that in a sum; beside the rounding
+    to bfloat16, whose own size the 64-bit results give.  A tenth more for chance; the mean of N errors lies within 5 / sqrt N of 0."""
+    g = gen(k + 1)
+    x, w = randn(g, m, k).to(DT["e4m3"]), randn(g, n, k).to(DT["e4m3"])
+    exact = x.double() @ w.double().t().contiguous()
+    off = crnn.linear(x, w).double() - exact
+    pad = (-k) % 8
+    top = [torch.nn.functional.pad(t.float().abs(), (0, pad)).view(t.shape[0], -1, 8).amax(2).square().mean() for t in (x, w)]
+    lost = (k * float(top[0] * top[1]) / 3) ** 0.5 * 2.0 ** -13
+    own = exact.to(torch.bfloat16).double() - exact
+    rms = lambda t: float(t.square().mean() ** 0.5)
+    print("%d x %d x %d: rms %.4g, rounding alone %.4g, allowed for the instructions %.4g; mean %.3g of %.3g" % (m, k, n, rms(off), rms(own), lost, float(off.mean()), rms(exact)))
+    assert rms(off) <= 1.1 * (rms(own) ** 2 + lost ** 2) ** 0.5
+    assert abs(float(off.mean())) <= 5 * rms(off) / (m * n) ** 0.5
+
+
+@pytest.mark.parametrize("m, k, n", [(9, 4096, 500), (48, 8192, 200), (300, 2048, 300), (800, 4096, 1100), (300, 2049, 300)])
+def test_linear_8_bits_operands_of_one_sign(crnn, m, k, n):
+    """What the instructions cut off products of one sign adds up: less than 2^-13 of the largest of eight, g, a product."""
+    g = gen(k + 2)
+    x, w = randn(g, m, k).abs().to(DT["e4m3"]), randn(g, n, k).abs().to(DT["e4m3"])
+    exact = x.double() @ w.double().t().contiguous()
+    off = crnn.linear(x, w).double() - exact
+    pad = (-k) % 8
+    xg, wg = (torch.nn.functional.pad(t.double(), (0, pad)).view(t.shape[0], -1, 8).amax(2) for t in (x, w))
+    lost = 8 * 2.0 ** -13 * (xg @ wg.t().contiguous())
+    own = exact.to(torch.bfloat16).double() - exact
+    print("%d x %d x %d: mean error %.3g of %.4g, allowed %.3g; rms %.4g, rounding alone %.4g" % (m, k, n, float(off.mean()), float(exact.mean()), float(lost.mean()), float(off.square().mean() ** 0.5), float(own.square().mean() ** 0.5)))
+    # (the last term: 2^-23 for each of the sums' additions, and a result that crosses the middle of two values moves a whole step)
+    assert (off.abs() <= lost + (k + 8) * 2.0 ** -23 * exact + 2.0 ** -8 * exact * (1 + 2.0 ** -8)).all()
+    assert abs(float((off - own).mean())) <= float(lost.mean()) + (k + 8) * 2.0 ** -23 * float(exact.mean()) + 5 * float(own.square().mean() ** 0.5) * (2 / (m * n)) ** 0.5
