@@ -130,6 +130,8 @@ class SequenceOps(object):
         float32 or bfloat16: of the result and the residual (default: x's, bfloat16 for float8).  ``out`` may be the
         residual itself."""
         torch = _t or _torch()
+        if x is None or w is None:
+            raise TypeError("linear: x or w is missing")
         stream = self._tensors("linear", ("x", "w", "bias", "residual", "x_scale", "w_scale", "out"), (x, w, bias, residual, x_scale, w_scale, out))
         dt = x.dtype
         if w.dim() != 2 or w.dtype is not dt or dt not in _types:
@@ -176,12 +178,16 @@ class SequenceOps(object):
         ``scale``, one float32 per row with y = values * scale (the operands ``linear`` takes).  ``sum`` is t in x's type;
         without a residual None.  ``sum_out`` may be x or residual themselves, ``out`` too where the types agree."""
         torch = _t or _torch()
+        if x is None or gain is None:
+            raise TypeError("rms_norm: x or gain is missing")
         stream = self._tensors("rms_norm", ("x", "gain", "residual", "out", "sum_out"), (x, gain, residual, out, sum_out))
         dt, shape = x.dtype, x.shape
         if len(shape) < 1 or (dt is not _f32 and dt is not _bf16):
             raise ValueError("rms_norm: x has to be float32 or bfloat16 [..., n], got %s %s" % (dt, tuple(shape)))
         n = shape[-1]
         self._vector("rms_norm", "gain", gain, n)
+        if not hasattr(eps, "__float__"):
+            raise TypeError("rms_norm: eps is not a number, got %r" % (eps,))
         if out_dtype is None:
             out_dtype = out.dtype if out is not None else dt
         if out_dtype is not dt and out_dtype is not _e4m3:
@@ -222,6 +228,8 @@ class SequenceOps(object):
         ``mask`` bool or uint8 [b, s]: the keys that count (both may be given).  A row without any key gives zeros; what the
         left-out keys hold is never looked at.  ``scale``: d ** -0.5."""
         torch = _t or _torch()
+        if q is None or k is None or v is None:
+            raise TypeError("cross_attention: q, k or v is missing")
         stream = self._tensors("cross_attention", ("q", "k", "v", "lengths", "mask", "out"), (q, k, v, lengths, mask, out))
         qs, ks, dt = q.shape, k.shape, q.dtype
         if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[0] != qs[0] or ks[3] != qs[3]:
@@ -244,7 +252,10 @@ class SequenceOps(object):
         o1, o2, o3, _ = out.stride()
         args = (b, t, s, heads, kv_heads, d, _types[dt], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q1, q2, q3, k1, k2, k3, v1, v2, v3,
                 o1, o2, o3, _ptr(lengths), _ptr(mask), mask.stride(0) if mask is not None else 0)
-        scale = d ** -0.5 if scale is None else scale
+        if scale is None:
+            scale = d ** -0.5
+        elif not hasattr(scale, "__float__"):
+            raise TypeError("cross_attention: scale is not a number, got %r" % (scale,))
         a = _CROSS_ATTENTION.pack(*args, 0, 0, scale, 0)
         need = self._lib.crnn_cross_attention_workspace(self._h, a)
         if need:
@@ -261,6 +272,8 @@ class SequenceOps(object):
         int32 [n]), T = crnn_out_len(w).  ``widths``: valid width of each line (host).  States are what the classifier reads
         (float32, bfloat16 with precision='bf16'), zeros behind a line's own length; ready on torch's current stream."""
         torch = _torch()
+        if lines is None:
+            raise TypeError("line_states: lines are missing")
         stream = self._tensors("line_states", ("lines",), (lines,))
         if lines.dtype is not torch.uint8 or lines.dim() != 3 or lines.shape[1] != 32 or not lines.is_contiguous() or lines.shape[0] == 0:
             raise ValueError("line_states: expected contiguous uint8 [n, 32, w], got %s %s" % (lines.dtype, tuple(lines.shape)))

@@ -1,6 +1,7 @@
 """Argument checks of the sequence operators and the error bounds their tests use: no GPU."""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -258,3 +259,18 @@ def test_line_attention_checks_head_size_biases_and_scales():
                       (q8, {"q.scale": torch.ones(32).double()})):
         with pytest.raises(ValueError, match=next(iter(change))):
             LineAttention(None, dict(w, **change), heads=4)
+
+
+def test_what_does_not_fit_is_a_type_or_value_error(monkeypatch):
+    """Also a tensor that is missing, and what is no number."""
+    face = host_face(monkeypatch)
+    x, w, q = torch.ones(4, 16), torch.ones(8, 16), torch.ones(2, 3, 4, 8)
+    for call in (lambda: face.linear(None, w), lambda: face.linear(x, None), lambda: face.rms_norm(None, x[0]), lambda: face.rms_norm(x, None),
+                 lambda: face.cross_attention(None, q, q), lambda: face.cross_attention(q, None, q), lambda: face.cross_attention(q, q, None),
+                 lambda: face.line_states(None), lambda: face.rms_norm(x, x[0], eps=None), lambda: face.cross_attention(q, q, q, scale="1")):
+        with pytest.raises(TypeError):
+            call()
+    assert face._lib.calls == []
+    face.rms_norm(x, x[0], eps=np.float32(1e-5))
+    face.cross_attention(q, q, q, scale=torch.tensor(0.5))
+    assert face._lib.calls == ["crnn_rms_norm", "crnn_cross_attention_workspace", "crnn_cross_attention"]
