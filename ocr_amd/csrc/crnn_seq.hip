@@ -187,8 +187,9 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
 // slice: by then everybody has read this step's stage, and the loads for NST steps on go into it.  Steps past the end load zeros,
 // which keeps the count of loads in flight the same to the last step.  KG groups of waves take steps in turn and add up at the
 // end where tiles are few.
-// Bound by power where k is long (the chip runs at 1.6 to 1.9 GHz then): bf16 8192 x 8192 x 8192 844 us, 1300 TF/s, which is
-// what the library's product takes; 8 bits 18176 x 2048 x 2048 85 us, 1780 TF/s.  Where k is short, by the way in and out, which
+// Where k is long matrix instructions are busy 65 % of the time, at the 1.6 to 1.9 GHz that power leaves the chip then: bf16 8192 x
+// 8192 x 8192 828 to 844 us, 1300 to 1330 TF/s (the library's product in turn with it: 680 to 760); 8 bits 18176 x 2048 x 2048 81
+// to 85 us, 1830 TF/s.  Where k is short, by the way in and out, which
 // nothing hides: 18176 x k x 2048 takes 24 us and 30 more for each 512 of k, 14 of the 24 being the rows that leave.  (One workgroup a CU
 // that loads its next tile before it writes the last: 59 us for k = 512, this 56.)
 // ---------------------------------------------------------------------------
@@ -227,10 +228,10 @@ template <> struct Slice<CRNN_FP32> {   // one 16-byte chunk a lane: four v_mfma
 // either sign (bits of them below 2^-126 may be lost, what a product with subnormal operands taken as 0 loses of a whole
 // operand).  m is at most 2^-8 of x and l 2^-17.  Of the nine products the six largest are multiplied (v_mfma_f32_32x32x16_bf16 at 16
 // times the rate of the f32 instructions); the others come to at most 2^-24 of the product, of either sign.  (Parts that are cut off
-// have x's sign and are twice as large: up to 7.8 2^-24 of a product are missing then, which sums do not average out.  It took
-// 666 us where this takes 722; with v_cvt_pk_bf16_f32 4544 x 512 x 512 34 and 33.)  An infinity makes h infinite and m NaN, a NaN l, and
+// have x's sign and are twice as large: up to 7.8 2^-24 of a product are missing then, which sums do not average out.  They took
+// 719 us where these take 779; with v_cvt_pk_bf16_f32 4544 x 512 x 512 34 and 33.)  An infinity makes h infinite and m NaN, a NaN l, and
 // values near the largest may overflow on the way: results that are not finite are computed again (finite_sums).  4096 x 4096 x
-// 4096 722 us, 190 TF/s; on the f32 instructions 1057 us, 130 TF/s.
+// 4096 722 to 779 us by box, 176 to 190 TF/s; on the f32 instructions 1057 us, 130 TF/s.
 struct Parts {
   bf16x8 p[3];
 };
@@ -879,9 +880,10 @@ static bool linear_tiles(const crnn_linear_args& a, hipStream_t s) {
     if (c3 <= c2) return linear_tile<IN, OUT, 3, 2, 4, 2>(a, s), true;
   }
   if (small >= 256) linear_tile<IN, OUT, 2, 2, 2, 2>(a, s);
-  // (fp32: a larger tile halves the work of splitting; two groups of waves over k where it leaves CUs with one workgroup.
-  // 8000 x 512 x 512, 252 tiles, 33 us, in 64 x 64 ones 39; 4544 x 512 x 512, 144, 31 and 27, too few CUs have work)
-  else if (IN == CRNN_FP32 && small >= 192) linear_tile<IN, OUT, 2, 2, 2, 2, 2>(a, s);
+  // (fp32: a larger tile halves the work of splitting; two groups of waves over k where it leaves CUs with one workgroup.  It pays from
+  // where 64 x 64 ones come to more than two a CU, and where k is long enough to share: 8000 x 512 x 512, 252 tiles, 36 us, in 64 x 64
+  // ones 46; 4544 x 512 x 512, 144, 28 and 30; 4096 x 512 x 512, 128, 28 and 24; 4544 x 64 x 512 11.1 and 8.9)
+  else if (IN == CRNN_FP32 && small >= (a.k < 512 ? 192 : 129)) linear_tile<IN, OUT, 2, 2, 2, 2, 2>(a, s);
   // (few small tiles: four groups of waves share k.  64 x 2048 x 2048 9.2 us, without 12.5; 300 x 512 x 5530 20 us, without 11)
   else if (tiny <= 256) linear_tile<IN, OUT, 1, 1, 1, 3, 4>(a, s);
   else linear_tile<IN, OUT, 1, 1, 2, 3>(a, s);
@@ -1054,7 +1056,7 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(const crnn_rms_norm_a
 // Rows that fit the registers of one wave (TPR 64: four rows a workgroup) or one workgroup (TPR 256): x and the residual are
 // read once, everything else happens in registers.  A thread holds C groups of eight values, which it loads and stores whole at
 // whatever alignment rows have, one by one where the row ends; the gain stays in registers over the rows that a workgroup takes.
-// Bound by HBM: 18176 x 2048 bf16 with residual and sum to 8 bits 55 to 58 us (4.5 TB/s and more), 18176 x 8192 to bf16 219 us
+// Bound by HBM: 18176 x 2048 bf16 with residual and sum to 8 bits 56 to 61 us (4.5 TB/s and more), 18176 x 8192 to bf16 219 us
 // (5.4 TB/s); 18176 x 2047 to 8 bits 75 us, rows crossing cache lines.
 template <int IN, int OUT, int TPR, int C>
 __global__ __launch_bounds__(256) void rms_norm_kernel(const crnn_rms_norm_args a) {
@@ -1280,7 +1282,10 @@ struct SplitRow {
 // read at once -- 16 rows of K, 64 bytes of four rows of V -- over the 256 bytes that LDS serves in a cycle.  fp32 runs the same
 // way on v_mfma_f32_32x32x2_f32: a 16-byte chunk feeds four of them, register r of S^T is one's second operand, and V is read
 // value by value (its rows r and r + 4 half a row apart).  Keys that are left out are never loaded: their
-// offset lies outside the resource, LDS gets zeros, and their score is -inf.
+// offset lies outside the resource, LDS gets zeros, and their score is -inf.  bf16: p is rounded to bf16 for the second product, while
+// L adds it in 32 bits -- its matrix instructions take no wider operand beside bf16 values, and p in two parts would be half as
+// many products again.  Each p is off by at most 2^-8; the case below is 2.06e-3 of its result from 64 bits, 1.66e-3 being the
+// results' own rounding.
 // With nsplit > 1 workgroups share the keys of one row block and leave (O, M, L) for attention_join_kernel.
 // Bound by both products and the exponentials between them, which the two waves of a SIMD hardly ever do side by side (matrix
 // instructions are busy 38 % of the time, vector ones 46): bf16 8 x 1024 queries of 16 heads over 4096 keys of 4, head_dim 128,
